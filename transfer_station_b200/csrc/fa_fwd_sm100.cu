@@ -690,9 +690,11 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) mx[k] = fmax3(u2f(sr[k]), u2f(sr[8 + k]), u2f(sr[16 + k]));
 #pragma unroll
-                    for (int c = 24; c < 128; c += 16)
+                    for (int c = 24; c < 120; c += 16)
 #pragma unroll
                         for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], u2f(sr[c + k]), u2f(sr[c + 8 + k]));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) mx[k] = fmaxf(mx[k], u2f(sr[120 + k]));
                     mb = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(fmax3(mx[3], mx[4], mx[5]), mx[6], mx[7]));
                 } else {
                     const int nvalid = nv < 0 ? 0 : (int)nv;
