@@ -91,6 +91,14 @@ EXPORTS = {
     "attn_diag_plan": (ctypes.c_int, [ctypes.c_int] * 7 + [ctypes.POINTER(ctypes.c_int)]),
     "attn_diag_wait_timeout": (ctypes.c_int, [_u16p, _u16p, _u16p, _f32p] + [ctypes.c_int] * 4 +
                                [ctypes.c_void_p, ctypes.c_void_p]),
+    # include/attn_flash_mod.h
+    "attn_flash_mod_stream": (ctypes.c_int, [_u16p, _u16p, _u16p, ctypes.c_void_p] + [ctypes.c_int] * 7 +
+                              [ctypes.c_void_p] * 3),
+    "attn_flash_mod_paged_stream": (ctypes.c_int, [_u16p, _u16p, _u16p, ctypes.c_void_p, ctypes.c_void_p,
+                                                   ctypes.c_void_p] + [ctypes.c_int] * 6 + [ctypes.c_void_p] +
+                                    [ctypes.c_int] * 3 + [ctypes.c_void_p, ctypes.c_void_p]),
+    "attn_mask_ranges_stream": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int] * 4 +
+                                [ctypes.c_void_p] * 3),
     # include/attn_qkv_rope.h
     "attn_rope_table_stream": (ctypes.c_int, [_f32p, ctypes.c_int, ctypes.c_int, ctypes.c_double, ctypes.c_void_p]),
     "attn_qkv_rope_stream": (ctypes.c_int, [_u16p, ctypes.c_void_p, _f32p, ctypes.c_int, _u16p, _u16p, ctypes.c_float]
@@ -185,6 +193,48 @@ def attn_flash_paged_stream(Q, K_pages, V_pages, block_table, seq_lens, O, B, Hq
     return int(load_library().attn_flash_paged_stream(
         _ptr(Q), _ptr(K_pages), _ptr(V_pages), _ptr(block_table), _ptr(seq_lens), _ptr(O), B, Hq, Hkv, Sq, D,
         int(causal), page_size, num_pages, max_pages, _ptr(scratch), _stream_handle(stream)))
+
+
+class AttnMod(ctypes.Structure):
+    """struct attn_mod: how attention scores are modified (attn_mod() makes one from tensors)."""
+
+    _fields_ = [("softcap", ctypes.c_float), ("causal", ctypes.c_int), ("slopes", ctypes.c_void_p),
+                ("key_begin", ctypes.c_void_p), ("key_end", ctypes.c_void_p)]
+
+
+def attn_mod(softcap=0.0, causal=0, slopes=None, key_begin=None, key_end=None) -> AttnMod:
+    """Modified scores: softcap * tanh(s / softcap) when softcap > 0, minus slopes[h] * distance (fp32
+    [Hq]), keys limited to [key_begin, key_end) (int32 [B][Sq], each optional) and by causality. The
+    returned struct holds on to the tensors."""
+    mod = AttnMod(float(softcap), int(bool(causal)), _ptr(slopes), _ptr(key_begin), _ptr(key_end))
+    mod.tensors = (slopes, key_begin, key_end)
+    return mod
+
+
+def _mod_ref(mod):
+    return None if mod is None else ctypes.byref(mod)
+
+
+def attn_flash_mod_stream(Q, K, V, O, out_dtype, B, Hq, Hkv, Sq, Sk, D, mod, scratch, stream=None) -> int:
+    """Attention with modified scores (attn_mod(), or None): Q [B*Hq][Sq][D], K/V [B*Hkv][Sk][D] bf16
+    bits, O fp32 or bf16 bits by out_dtype. Returns the status."""
+    return int(load_library().attn_flash_mod_stream(_ptr(Q), _ptr(K), _ptr(V), _ptr(O), int(out_dtype), B, Hq, Hkv, Sq,
+                                                     Sk, D, _mod_ref(mod), _ptr(scratch), _stream_handle(stream)))
+
+
+def attn_flash_mod_paged_stream(Q, K_pages, V_pages, block_table, seq_lens, O, out_dtype, B, Hq, Hkv, Sq, D, mod,
+                                page_size, num_pages, max_pages, scratch, stream=None) -> int:
+    """attn_flash_paged_stream with modified scores and a choice of output type. Returns the status."""
+    return int(load_library().attn_flash_mod_paged_stream(
+        _ptr(Q), _ptr(K_pages), _ptr(V_pages), _ptr(block_table), _ptr(seq_lens), _ptr(O), int(out_dtype), B, Hq, Hkv,
+        Sq, D, _mod_ref(mod), page_size, num_pages, max_pages, _ptr(scratch), _stream_handle(stream)))
+
+
+def attn_mask_ranges_stream(cu_docs, prefix, n_docs, S, causal, window, key_begin, key_end, stream=None) -> int:
+    """Key ranges int32 [S] of documents packed into S tokens (cu_docs int32 [n_docs + 1], prefix int32
+    [n_docs] or None, window 0 for none). Returns the status."""
+    return int(load_library().attn_mask_ranges_stream(_ptr(cu_docs), _ptr(prefix), n_docs, S, int(bool(causal)), window,
+                                                       _ptr(key_begin), _ptr(key_end), _stream_handle(stream)))
 
 
 def attn_rope_table_stream(cos_sin, max_pos, rot, theta, stream=None) -> int:
@@ -340,4 +390,4 @@ def attn_flash_combine_stream(m, l, acc, nparts, rows, D, O, stream=None) -> int
 
 
 __all__ = [n for n in dir() if n.startswith("attn_") or n.startswith("ATTN_")] + [
-    "AttnError", "load_library", "strerror", "LIB_PATH", "EXPORTS"]
+    "AttnError", "AttnMod", "load_library", "strerror", "LIB_PATH", "EXPORTS"]

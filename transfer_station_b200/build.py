@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -28,7 +29,8 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 CC = os.environ.get("CC", "gcc")
 CC_FLAGS = ["-O2", "-std=c11", "-fPIC", "-Wall", "-Wextra"]
 
-CU_SOURCES = ["fa_fwd_sm100.cu", "fa_aux.cu", "fa_noalloc.cu", "fa_diag.cu", "fa_peer.cu", "qkv_rope.cu"]
+CU_SOURCES = ["fa_fwd_sm100.cu", "fa_aux.cu", "fa_noalloc.cu", "fa_diag.cu", "fa_peer.cu", "qkv_rope.cu", "fa_mod.cu",
+              "fa_mod_range.cu", "fa_mod_cap.cu", "fa_mod_bias.cu", "fa_mod_capbias.cu"]
 C_SOURCES = ["attn_flash.c", "attn_qkv_rope.c"]
 
 
@@ -59,17 +61,19 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         return out
     OBJDIR.mkdir(parents=True, exist_ok=True)
     LIBDIR.mkdir(parents=True, exist_ok=True)
-    objs = []
+    objs, cmds = [], []
     inc = ["-I", str(INCLUDE), "-I", str(CSRC)]
     for src in CU_SOURCES:
         obj = OBJDIR / (Path(src).stem + ".o")
         extra = ["-Xptxas", "-v"] if ptxas_verbose else []
-        _run([NVCC, *ARCH, *NVCC_FLAGS, *extra, *inc, "-c", str(CSRC / src), "-o", str(obj)], verbose or ptxas_verbose)
+        cmds.append([NVCC, *ARCH, *NVCC_FLAGS, *extra, *inc, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(str(obj))
     for src in C_SOURCES:
         obj = OBJDIR / (Path(src).stem + ".o")
-        _run([CC, *CC_FLAGS, *inc, "-c", str(CSRC / src), "-o", str(obj)], verbose)
+        cmds.append([CC, *CC_FLAGS, *inc, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(str(obj))
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:  # the sources are independent
+        list(pool.map(lambda c: _run(c, verbose or ptxas_verbose), cmds))
     tmp = out.with_suffix(".so.tmp")
     _run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objs, "-lm"], verbose)
     os.replace(tmp, out)

@@ -13,6 +13,7 @@
 
 #include "attn_flash.h"
 #include "attn_flash_diag.h"
+#include "attn_flash_mod.h"
 #include "fa_launch.h"
 
 /* flash.c:641-647: a bk the caller did not also size scratch with must fail loudly, never
@@ -103,7 +104,8 @@ static void ts_plan_core(fa_problem *p, int tc, int sms, int ctas) {
     if (sms < 1) sms = 1;
     p->n_direct = 0;
     p->row_base = 0;
-    long long cap = rows > 0 ? (long long)ATTN_PARTIAL_ROWS / rows : 0;
+    const long long room = p->part_cap > 0 ? p->part_cap : ATTN_PARTIAL_ROWS;
+    long long cap = rows > 0 ? room / rows : 0;
     int smax = nblk / 2;
     if (smax > cap) smax = (int)cap;
     if (smax > 256) smax = 256;
@@ -133,7 +135,7 @@ static void ts_plan_core(fa_problem *p, int tc, int sms, int ctas) {
     const long long row_base = (long long)(u0 / tiles) * rows_per_kv + (long long)(u0 % tiles) * ur;
     int s = sms / L;
     if (s > nblk / 2) s = nblk / 2;
-    while (s >= 2 && (rows - row_base) * s > ATTN_PARTIAL_ROWS) --s;
+    while (s >= 2 && (rows - row_base) * s > room) --s;
     if (s < 2) return;
     bps = (nblk + s - 1) / s;
     p->nsplit = (nblk + bps - 1) / bps;
@@ -251,10 +253,10 @@ static int ts_page_size_ok(int ps) {
     return ps > 0 && ps % ATTN_GPU_KEY_TILE == 0;
 }
 
-int attn_flash_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const uint16_t *V_pages,
-                            const int *block_table, const int *seq_lens, float *O, int B, int Hq, int Hkv, int Sq,
-                            int D, int causal, int page_size, int num_pages, int max_pages, void *scratch,
-                            void *stream) {
+/* The argument checks of a paged call. */
+static int ts_paged_check(const void *Q, const void *K_pages, const void *V_pages, const int *block_table,
+                          const int *seq_lens, const void *O, int B, int Hq, int Hkv, int Sq, int D, int page_size,
+                          int num_pages, int max_pages, const void *scratch) {
     if (!Q || !K_pages || !V_pages || !block_table || !seq_lens || !O || !scratch) return ATTN_ERR_ARGS;
     if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || Sq < 1 || num_pages < 1 || max_pages < 1)
         return ATTN_ERR_ARGS;
@@ -265,6 +267,16 @@ int attn_flash_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const ui
     if (((uintptr_t)Q | (uintptr_t)K_pages | (uintptr_t)V_pages | (uintptr_t)O | (uintptr_t)scratch) & 15u)
         return ATTN_ERR_ALIGN;
     if (ts_cc_major() != 10) return ATTN_ERR_NOT_SM100;
+    return ATTN_OK;
+}
+
+int attn_flash_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const uint16_t *V_pages,
+                            const int *block_table, const int *seq_lens, float *O, int B, int Hq, int Hkv, int Sq,
+                            int D, int causal, int page_size, int num_pages, int max_pages, void *scratch,
+                            void *stream) {
+    const int rc = ts_paged_check(Q, K_pages, V_pages, block_table, seq_lens, O, B, Hq, Hkv, Sq, D, page_size, num_pages,
+                                  max_pages, scratch);
+    if (rc != ATTN_OK) return rc;
     fa_problem p;
     ts_fill(&p, Q, K_pages, V_pages, B * Hq, B * Hkv, Sq, max_pages * page_size, D, causal, 0);
     p.O = O;
@@ -277,6 +289,105 @@ int attn_flash_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const ui
     p.hkv_local = Hkv;
     if (!ts_tc_supported(&p)) return ATTN_ERR_ARGS;
     return ts_run(&p, scratch, stream);
+}
+
+/* Checks a call's modifiers and sets the problem's (Hkv kv heads per sequence). A plain call keeps
+ * mod 0 and takes the plain kernels. */
+static int ts_set_mod(fa_problem *p, const attn_mod *mod, int Hkv) {
+    p->hkv_local = Hkv;
+    if (!mod) return ATTN_OK;
+    p->causal = mod->causal ? 1 : 0;
+    const float cap = mod->softcap;
+    if (!(cap == 0.0f || (cap >= ATTN_SOFTCAP_MIN && cap <= ATTN_SOFTCAP_MAX))) return ATTN_ERR_ARGS;
+    if ((((uintptr_t)mod->slopes) | ((uintptr_t)mod->key_begin) | ((uintptr_t)mod->key_end)) & 3u) return ATTN_ERR_ALIGN;
+    p->key_begin = mod->key_begin;
+    p->key_end = mod->key_end;
+    p->slopes = mod->slopes;
+    if (cap > 0.0f) {
+        p->cap_in = 1.0f / (cap * sqrtf((float)p->D));
+        p->cap_out = cap * 1.4426950408889634f;
+    }
+    if (cap > 0.0f || mod->slopes)
+        p->mod = cap > 0.0f ? (mod->slopes ? 4 : 2) : 3;
+    else if (mod->key_begin || mod->key_end)
+        p->mod = 1;
+    return ATTN_OK;
+}
+
+/* Query positions a unit's ranges are read from by the kernel itself; longer calls get their bounds
+ * from a kernel of their own first (about 2 us, against 256 dependent reads per unit and role). */
+#define TS_MOD_INLINE_ROWS 8
+
+/* Runs a problem with modified scores. The bounds of the units' ranges sit at the end of the scratch
+ * block's partial accumulators, which the plan then uses less of. */
+static int ts_run_mod(fa_problem *p, void *scratch, void *stream) {
+    if (p->mod && (p->key_begin || p->key_end) && p->Sq > TS_MOD_INLINE_ROWS && ts_tc_supported(p)) {
+        ts_scratch s;
+        ts_scratch_layout(scratch, p->D, &s);
+        const size_t units = (size_t)(p->Hkv / p->hkv_local) * (size_t)(ts_tc_ctas_per_split(p) / p->Hkv);
+        const size_t row_bytes = (size_t)p->D * sizeof(float);
+        const size_t taken = (units * 4 * sizeof(int) + row_bytes - 1) / row_bytes + 1;
+        if (taken <= ATTN_PARTIAL_ROWS / 2) { /* else: the kernel reads the ranges itself */
+            p->part_cap = ATTN_PARTIAL_ROWS - (int)taken;
+            /* 16-byte aligned, within the rows taken (one more than the bounds fill) */
+            p->bounds = (int *)(((uintptr_t)(s.acc + (size_t)p->part_cap * (size_t)p->D) + 15u) & ~(uintptr_t)15u);
+        }
+    }
+    return ts_run(p, scratch, stream);
+}
+
+int attn_flash_mod_stream(const uint16_t *Q, const uint16_t *K, const uint16_t *V, void *O, int out_dtype, int B,
+                          int Hq, int Hkv, int Sq, int Sk, int D, const attn_mod *mod, void *scratch, void *stream) {
+    if (!O || (out_dtype != ATTN_OUT_F32 && out_dtype != ATTN_OUT_BF16) || B < 1 || Hq < 1 || Hkv < 1)
+        return ATTN_ERR_ARGS;
+    if ((long long)B * Hq > 0x7fffffffLL) return ATTN_ERR_ARGS;
+    fa_problem p;
+    ts_fill(&p, Q, K, V, B * Hq, B * Hkv, Sq, Sk, D < 1 ? 1 : D, 0, 0);
+    int rc = ts_set_mod(&p, mod, Hkv);
+    if (rc == ATTN_ERR_ARGS || Hq % Hkv != 0) return ATTN_ERR_ARGS;
+    const int valid = ts_validate(Q, K, V, B * Hq, B * Hkv, Sq, Sk, D, scratch);
+    if (valid == ATTN_ERR_ARGS) return valid;
+    if (rc != ATTN_OK) return rc;
+    if (valid != ATTN_OK) return valid;
+    p.O = (float *)O;
+    p.o_bf16 = out_dtype == ATTN_OUT_BF16;
+    return ts_run_mod(&p, scratch, stream);
+}
+
+int attn_flash_mod_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const uint16_t *V_pages,
+                                const int *block_table, const int *seq_lens, void *O, int out_dtype, int B, int Hq,
+                                int Hkv, int Sq, int D, const attn_mod *mod, int page_size, int num_pages,
+                                int max_pages, void *scratch, void *stream) {
+    if (out_dtype != ATTN_OUT_F32 && out_dtype != ATTN_OUT_BF16) return ATTN_ERR_ARGS;
+    int rc = ts_paged_check(Q, K_pages, V_pages, block_table, seq_lens, O, B, Hq, Hkv, Sq, D, page_size, num_pages,
+                            max_pages, scratch);
+    if (rc == ATTN_ERR_ARGS) return rc;
+    fa_problem p;
+    ts_fill(&p, Q, K_pages, V_pages, B * Hq, B * Hkv, Sq, max_pages * page_size, D, 0, 0);
+    const int mrc = ts_set_mod(&p, mod, Hkv);
+    if (mrc == ATTN_ERR_ARGS) return mrc;
+    if (rc != ATTN_OK) return rc;
+    if (mrc != ATTN_OK) return mrc;
+    p.O = (float *)O;
+    p.o_bf16 = out_dtype == ATTN_OUT_BF16;
+    p.paged = 1;
+    p.block_table = block_table;
+    p.seq_lens = seq_lens;
+    p.page_size = page_size;
+    p.max_pages = max_pages;
+    p.num_pages = num_pages;
+    if (!ts_tc_supported(&p)) return ATTN_ERR_ARGS;
+    return ts_run_mod(&p, scratch, stream);
+}
+
+int attn_mask_ranges_stream(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,
+                            int *key_begin, int *key_end, void *stream) {
+    if (!cu_docs || !key_begin || !key_end || n_docs < 1 || S < 1 || window < 0 || (window > 0 && prefix))
+        return ATTN_ERR_ARGS;
+    if ((((uintptr_t)cu_docs) | ((uintptr_t)prefix) | ((uintptr_t)key_begin) | ((uintptr_t)key_end)) & 3u)
+        return ATTN_ERR_ALIGN;
+    if (ts_cc_major() != 10) return ATTN_ERR_NOT_SM100;
+    return ts_launch_mask_ranges(cu_docs, prefix, n_docs, S, causal ? 1 : 0, window, key_begin, key_end, stream);
 }
 
 int attn_flash_partial_stream(const uint16_t *Q, const uint16_t *K, const uint16_t *V, float *m, float *l,

@@ -52,10 +52,16 @@ struct SimtParams {
     int Hq, Hkv, Sq, Sk, Sk_total, k_begin, D, causal, v_prepacked;
     int keys_per_split, partial, o_bf16;
     float scale_log2;
+    // modified scores (attn_flash_mod_stream), as fa_problem's
+    const int *key_begin, *key_end;
+    const float *slopes;
+    float cap_in, cap_out;
+    int hkv_local;
 };
 
 constexpr int kSimtMaxU = ATTN_D_MAX / 32;  // columns per lane
 
+template <bool MOD>
 __global__ void __launch_bounds__(256) fa_simt_kernel(const SimtParams p) {
     const int lane = threadIdx.x & 31;
     const long long total_rows = (long long)p.Hq * p.Sq;
@@ -67,7 +73,20 @@ __global__ void __launch_bounds__(256) fa_simt_kernel(const SimtParams p) {
     const int kb0 = split * p.keys_per_split;
     const int kb1 = min(p.Sk, kb0 + p.keys_per_split);
     long long lim = p.causal ? ((long long)p.Sk_total - p.Sq + i - p.k_begin) : (long long)(p.Sk - 1);
-    const int kend = (int)max((long long)kb0, min((long long)kb1, lim + 1));
+    int kbeg = kb0, kend = (int)max((long long)kb0, min((long long)kb1, lim + 1));
+    float slope2 = 0.f;
+    int qpos = 0, near = 0;
+    if constexpr (MOD) {
+        int lo = 0, hi = p.causal ? (int)max(0ll, min((long long)p.Sk, lim + 1)) : p.Sk;
+        const size_t at = (size_t)(kv / p.hkv_local) * p.Sq + i;
+        if (p.key_begin) lo = min(max(0, p.key_begin[at]), p.Sk);
+        if (p.key_end) hi = max(0, min(hi, p.key_end[at]));
+        qpos = p.Sk_total - p.Sq + i;
+        near = max(0, max(lo - qpos, qpos - (hi - 1)));  // the nearest key the row sees
+        if (p.slopes) slope2 = p.slopes[h % (p.hkv_local * (p.Hq / p.Hkv))] * 1.4426950408889634f;
+        kbeg = max(kb0, lo);
+        kend = min(kend, hi);
+    }
 
     float q[kSimtMaxU], acc[kSimtMaxU];
 #pragma unroll
@@ -79,7 +98,7 @@ __global__ void __launch_bounds__(256) fa_simt_kernel(const SimtParams p) {
     float m = -INFINITY, l = 0.f;
     const uint16_t *Kh = p.K + (size_t)kv * p.Sk * p.D;
     const uint16_t *Vh = p.V + (size_t)kv * p.Sk * p.D;
-    for (int k = kb0; k < kend; ++k) {
+    for (int k = kbeg; k < kend; ++k) {
         float part = 0.f;
 #pragma unroll
         for (int u = 0; u < kSimtMaxU; ++u) {
@@ -88,7 +107,12 @@ __global__ void __launch_bounds__(256) fa_simt_kernel(const SimtParams p) {
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        const float s = part * p.scale_log2;
+        float s = part * p.scale_log2;
+        if constexpr (MOD) {
+            if (p.cap_out > 0.f) s = p.cap_out * tanhf(part * p.cap_in);
+            if (p.slopes) s -= slope2 * (float)(abs(k - qpos) - near);
+            if (s == -INFINITY) continue;  // weighs nothing, and would turn the first maximum into NaN
+        }
         if (s > m) {
             const float alpha = (m == -INFINITY) ? 0.f : ex2f(m - s);
             l *= alpha;
@@ -353,7 +377,16 @@ static int launch_simt(const fa_problem *P, void *stream, int partial) {
     const long long rows = (long long)P->Hq * P->Sq;
     const int warps = 8;
     dim3 grid((unsigned)((rows + warps - 1) / warps), P->nsplit);
-    ts::fa_simt_kernel<<<grid, 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(s);
+    s.key_begin = P->key_begin;
+    s.key_end = P->key_end;
+    s.slopes = P->slopes;
+    s.cap_in = P->cap_in;
+    s.cap_out = P->cap_out;
+    s.hkv_local = P->hkv_local > 0 ? P->hkv_local : 1;
+    if (P->mod)
+        ts::fa_simt_kernel<true><<<grid, 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(s);
+    else
+        ts::fa_simt_kernel<false><<<grid, 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(s);
     if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
     ts_count_launch();
     return ATTN_OK;
@@ -365,7 +398,11 @@ extern "C" int ts_launch_attention_pieces(const fa_problem *P, void *stream) {
 
 extern "C" int ts_launch_attention(const fa_problem *P, void *stream) {
     const bool tc = ts_tc_supported(P) != 0;
-    int rc = tc ? ts_launch_tc(P, stream) : launch_simt(P, stream, (P->nsplit > 1 || P->write_partials) ? 1 : 0);
+    if (tc && P->mod && P->bounds) {
+        const int rc = ts_launch_mod_bounds(P, stream);
+        if (rc != ATTN_OK) return rc;
+    }
+    int rc = tc ? (P->mod ? ts_launch_tc_mod(P, stream) : ts_launch_tc(P, stream)) : launch_simt(P, stream, (P->nsplit > 1 || P->write_partials) ? 1 : 0);
     if (rc != ATTN_OK || P->nsplit <= 1) return rc;
     // merge the key pieces of the split rows [base, Hq*Sq) (all rows on the general path)
     const int rows = P->Hq * P->Sq;

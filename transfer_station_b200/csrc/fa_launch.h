@@ -51,6 +51,16 @@ typedef struct fa_problem {
      * kernel clears it itself (CTA 0 zeroes status[0], then stores this value in status[1];
      * error reports wait for that store), so no memset has to sit between two launches. */
     unsigned status_gen;
+    /* Modified scores (attn_flash_mod_stream; mod 0: none): 1 key ranges only, 2 cap, 3 distance
+     * bias, 4 both. Key ranges [B][Sq] (either may be NULL) apply with every mod; kv head index =
+     * b * hkv_local + kv_local. bounds: scratch room for the per-unit range bounds, or NULL (the
+     * kernel then reads a unit's ranges itself). */
+    int mod;
+    const int *key_begin, *key_end;
+    int *bounds;
+    const float *slopes;       /* [Hq of one sequence] */
+    float cap_in, cap_out;     /* 1 / (cap * sqrt(D)), cap * log2(e) */
+    int part_cap;              /* partial rows the plan may use (0: ATTN_PARTIAL_ROWS) */
 } fa_problem;
 
 /* Number of SMs of the current device (cached). */
@@ -67,6 +77,14 @@ int ts_tc_unit_rows(const fa_problem *p);
 /* Launch the main kernel (tcgen05 or SIMT path chosen inside) plus, when nsplit > 1 and
  * !write_partials, the combine kernel. Returns 0 or a negative ATTN_ERR_* code. */
 int ts_launch_attention(const fa_problem *p, void *stream);
+
+/* Fill p->bounds (one int pair per sequence and row tile of a kv head) from the key ranges, and the
+ * tensor-core launch with modified scores. */
+int ts_launch_mod_bounds(const fa_problem *p, void *stream);
+int ts_launch_tc_mod(const fa_problem *p, void *stream);
+/* Key ranges of packed documents (fa_mod.cu), see attn_mask_ranges_stream. */
+int ts_launch_mask_ranges(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,
+                          int *key_begin, int *key_end, void *stream);
 
 /* Launch the combine kernel alone on partial arrays. */
 int ts_launch_combine(const float *m, const float *l, const float *acc, int nparts, int rows, int D,

@@ -83,6 +83,23 @@ __device__ __forceinline__ unsigned ld_acquire_gpu(const unsigned *p) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads of what the previous grid of the stream may have written: volatile, so that none moves above
+// pdl_wait (the __ldg family is not ordered against it).
+__device__ __forceinline__ int ld_plan(const int *p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_plan(const float *p) { return __int_as_float(ld_plan(reinterpret_cast<const int *>(p))); }
+__device__ __forceinline__ int4 ld_plan(const int4 *p) {
+    int4 v;
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+
 // ORs `code` into the status word status[0]. gen == 0: the host cleared the word before the
 // launch. gen != 0: the kernel clears it itself -- CTA 0 zeroes status[0], then publishes gen in
 // status[1] -- so a report first waits (bounded) until that clear is visible, and the clear can
