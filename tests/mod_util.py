@@ -25,10 +25,14 @@ def visible(B, Sq, lens, causal, begin=None, end=None, Sk=None, dev="cuda"):
     return seen
 
 
-def attend(q, k, v, seen, lens, cap=0.0, slopes=None, p_half=2.0 ** -8, out=torch.float32):
+def attend(q, k, v, seen, lens, cap=0.0, slopes=None, p_half=2.0 ** -8, out=torch.float32, p_abs=0.0):
     """64-bit attention and a bound on each element's error. q [B][Hq][Sq][D], k and v [B][Hkv][Sk][D] (any
     float type; exact values), seen [B][Sq][Sk]. The bound counts
       - P rounded to 1 / p_half steps: p_half * A, A = sum_j p_j |v_j|
+      - p_abs per key, where P's type has a smallest step (fp16: 2^-24). The 4-bit kernel's weights are
+        2^(z - m) with the largest at least 2^7 (m is a maximum less 7, and only ever replaced by a larger
+        one), so l >= 2^7 and half of that step is 2^-25 / 2^7 = 2^-32 of l; a merge of partials scales an
+        error by what it scales the partial's weights, and the partial with the largest m keeps l >= 2^7
       - scores: D products and D sums in 32 bits (2^-23 each on the tensor cores) of size |q||k|; scale,
         cap and bias a few roundings and the tanh fit (1e-6 relative in all); an error e of a score moves
         a weight by the factor 1 + e and the sum of weights by as much: 2 e A
@@ -74,4 +78,6 @@ def attend(q, k, v, seen, lens, cap=0.0, slopes=None, p_half=2.0 ** -8, out=torc
             e = D * 2.0 ** -23 * size + 1e-6 * torch.where(sb, big, torch.zeros_like(big)).amax(1, keepdim=True)
             A = p @ vv.abs()
             tol[b, h] = (p_half + 2 * e + 2.0 ** -17) * A + HALF[out] * o[b, h].abs() + 1e-30
+            if p_abs:
+                tol[b, h] += p_abs * (sb.double() @ vv.abs())
     return o, tol

@@ -2,7 +2,9 @@
 
 The product is the in-tree shared library ``lib/libattn_flash_b200.so`` (C host layer +
 tcgen05/TMA/TMEM CUDA kernels) whose entry points are declared in ``include/attn_flash.h``
-(the attention path) and ``include/attn_qkv_rope.h`` (the QKV producer before it).
+(the attention path), ``include/attn_flash_mod.h`` (attention with modified scores),
+``include/attn_qkv_rope.h`` (the QKV producer before it) and ``include/attn_kv4.h`` (the 4-bit
+key cache: its producer, its attention and its tokens back).
 This module is the thin Python mirror of that C ABI (ctypes), used by the tests and the
 benchmark: same names, same argument meaning, same error behaviour. It never computes
 anything itself -- if the library is missing it raises, there is no fallback.
@@ -30,6 +32,8 @@ ATTN_PEER_HANDLE_BYTES = 128
 
 ATTN_OUT_F32 = 0
 ATTN_OUT_BF16 = 1
+
+ATTN_KV4_GROUP = 32
 
 ATTN_ROPE_GPTJ = 0
 ATTN_ROPE_NEOX = 1
@@ -108,6 +112,13 @@ EXPORTS = {
                                                   ctypes.c_float] + [ctypes.c_int] * 7
                                    + [_u16p, _u16p, _u16p, ctypes.c_void_p] + [ctypes.c_int] * 3
                                    + [ctypes.c_void_p, ctypes.c_void_p]),
+    # include/attn_kv4.h
+    "attn_qkv_rope_kv4_stream": (ctypes.c_int, [_u16p, ctypes.c_void_p, _f32p, ctypes.c_int, _u16p, _u16p,
+                                                ctypes.c_float] + [ctypes.c_int] * 7 + [ctypes.c_void_p] * 6
+                                 + [ctypes.c_int] * 3 + [ctypes.c_void_p, ctypes.c_void_p]),
+    "attn_kv4_unpack_stream": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_int] * 7 + [ctypes.c_void_p] * 2),
+    "attn_flash_kv4_stream": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_int] * 6 + [ctypes.c_void_p] +
+                              [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2),
 }
 
 _lib = None
@@ -264,6 +275,36 @@ def attn_qkv_rope_paged_stream(qkv, positions, cos_sin, max_pos, q_norm_w, k_nor
         _ptr(qkv), _ptr(positions), _ptr(cos_sin), max_pos, _ptr(q_norm_w), _ptr(k_norm_w), float(eps), B, S, Hq,
         Hkv, D, rot, style, _ptr(Q), _ptr(K_pages), _ptr(V_pages), _ptr(block_table), page_size, num_pages,
         max_pages, _ptr(scratch), _stream_handle(stream)))
+
+
+def attn_qkv_rope_kv4_stream(qkv, positions, cos_sin, max_pos, q_norm_w, k_norm_w, eps, B, S, Hq, Hkv, D, rot, style, Q,
+                             K_codes, K_scales, V_codes, V_scales, block_table, page_size, num_pages, max_pages, scratch,
+                             stream=None) -> int:
+    """attn_qkv_rope_paged_stream into a 4-bit cache: code pools uint8 [num_pages][Hkv][page_size][D/2], scale
+    pools uint8 (E4M3) [num_pages][Hkv][page_size][D/32]. Returns the status."""
+    return int(load_library().attn_qkv_rope_kv4_stream(
+        _ptr(qkv), _ptr(positions), _ptr(cos_sin), max_pos, _ptr(q_norm_w), _ptr(k_norm_w), float(eps), B, S, Hq, Hkv, D,
+        rot, style, _ptr(Q), _ptr(K_codes), _ptr(K_scales), _ptr(V_codes), _ptr(V_scales), _ptr(block_table), page_size,
+        num_pages, max_pages, _ptr(scratch), _stream_handle(stream)))
+
+
+def attn_kv4_unpack_stream(K_codes, K_scales, V_codes, V_scales, block_table, positions, K, V, B, S, Hkv, D, page_size,
+                           num_pages, max_pages, scratch, stream=None) -> int:
+    """The 4-bit cache's tokens at positions int32 [B*S] as bf16 bits: K and V [B*Hkv][S][D]. Returns the
+    status."""
+    return int(load_library().attn_kv4_unpack_stream(
+        _ptr(K_codes), _ptr(K_scales), _ptr(V_codes), _ptr(V_scales), _ptr(block_table), _ptr(positions), _ptr(K),
+        _ptr(V), B, S, Hkv, D, page_size, num_pages, max_pages, _ptr(scratch), _stream_handle(stream)))
+
+
+def attn_flash_kv4_stream(Q, K_codes, K_scales, V_codes, V_scales, block_table, seq_lens, O, out_dtype, B, Hq, Hkv, Sq, D,
+                          mod, page_size, num_pages, max_pages, scratch, stream=None) -> int:
+    """Attention over the 4-bit paged cache (Q [B*Hq][Sq][D] bf16 bits, O fp32 or bf16 bits by out_dtype, mod from
+    attn_mod() or None). Returns the status."""
+    return int(load_library().attn_flash_kv4_stream(
+        _ptr(Q), _ptr(K_codes), _ptr(K_scales), _ptr(V_codes), _ptr(V_scales), _ptr(block_table), _ptr(seq_lens), _ptr(O),
+        int(out_dtype), B, Hq, Hkv, Sq, D, _mod_ref(mod), page_size, num_pages, max_pages, _ptr(scratch),
+        _stream_handle(stream)))
 
 
 def attn_flash_packed_floats(rows: int, D: int) -> int:

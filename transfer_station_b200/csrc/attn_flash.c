@@ -14,6 +14,7 @@
 #include "attn_flash.h"
 #include "attn_flash_diag.h"
 #include "attn_flash_mod.h"
+#include "attn_kv4.h"
 #include "fa_launch.h"
 
 /* flash.c:641-647: a bk the caller did not also size scratch with must fail loudly, never
@@ -377,6 +378,58 @@ int attn_flash_mod_paged_stream(const uint16_t *Q, const uint16_t *K_pages, cons
     p.num_pages = num_pages;
     if (!ts_tc_supported(&p)) return ATTN_ERR_ARGS;
     return ts_run_mod(&p, scratch, stream);
+}
+
+int attn_flash_kv4_stream(const uint16_t *Q, const uint8_t *K_codes, const uint8_t *K_scales, const uint8_t *V_codes,
+                          const uint8_t *V_scales, const int *block_table, const int *seq_lens, void *O, int out_dtype,
+                          int B, int Hq, int Hkv, int Sq, int D, const attn_mod *mod, int page_size, int num_pages,
+                          int max_pages, void *scratch, void *stream) {
+    if (!K_scales || !V_scales || (out_dtype != ATTN_OUT_F32 && out_dtype != ATTN_OUT_BF16)) return ATTN_ERR_ARGS;
+    if (D != 64 && D != 128) return ATTN_ERR_ARGS;
+    int rc = ts_paged_check(Q, K_codes, V_codes, block_table, seq_lens, O, B, Hq, Hkv, Sq, D, page_size, num_pages,
+                            max_pages, scratch);
+    if (rc == ATTN_ERR_ARGS) return rc;
+    if ((long long)page_size * max_pages > 0x7fffffffLL - 1024 || (long long)B * Hkv > 0x7fffffffLL) return ATTN_ERR_ARGS;
+    fa_problem f;
+    ts_fill(&f, Q, NULL, NULL, B * Hq, B * Hkv, Sq, max_pages * page_size, D, 0, 0);
+    const int mrc = ts_set_mod(&f, mod, Hkv);
+    if (mrc != ATTN_OK) return mrc;
+    if ((((uintptr_t)K_scales) | ((uintptr_t)V_scales)) & 15u) return ATTN_ERR_ALIGN;
+    if (rc != ATTN_OK) return rc;
+    ts_scratch s;
+    ts_scratch_layout(scratch, D, &s);
+    ts_kv4_problem P;
+    memset(&P, 0, sizeof P);
+    P.Q = Q;
+    P.k_codes = K_codes;
+    P.k_scales = K_scales;
+    P.v_codes = V_codes;
+    P.v_scales = V_scales;
+    P.block_table = block_table;
+    P.seq_lens = seq_lens;
+    P.O = O;
+    P.o_bf16 = out_dtype == ATTN_OUT_BF16;
+    P.B = B;
+    P.Hq = Hq;
+    P.Hkv = Hkv;
+    P.Sq = Sq;
+    P.D = D;
+    P.causal = f.causal;
+    P.page_size = page_size;
+    P.num_pages = num_pages;
+    P.max_pages = max_pages;
+    P.scale_log2 = f.scale_log2;
+    P.cap_in = f.cap_in;
+    P.cap_out = f.cap_out;
+    P.slopes = f.slopes;
+    P.key_begin = f.key_begin;
+    P.key_end = f.key_end;
+    P.status = s.status;
+    P.part_m = s.m;
+    P.part_l = s.l;
+    P.part_acc = s.acc;
+    P.part_rows = ATTN_PARTIAL_ROWS;
+    return ts_launch_kv4(&P, stream);
 }
 
 int attn_mask_ranges_stream(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,

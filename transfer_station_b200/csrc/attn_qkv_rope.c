@@ -5,7 +5,9 @@
 #include <math.h>
 #include <stdint.h>
 #include <stddef.h>
+#include <string.h>
 
+#include "attn_kv4.h"
 #include "attn_qkv_rope.h"
 #include "fa_launch.h"
 
@@ -58,6 +60,7 @@ static int ts_rope_fill(ts_rope_problem *P, const uint16_t *qkv, const int *posi
     P->max_pos = rot > 0 ? max_pos : INT_MAX;
     P->cache_len = 0;
     P->page_size = P->num_pages = P->max_pages = 0;
+    P->k_codes = P->k_scales = P->v_codes = P->v_scales = NULL;
     return ATTN_OK;
 }
 
@@ -98,4 +101,75 @@ int attn_qkv_rope_paged_stream(const uint16_t *qkv, const int *positions, const 
     P.num_pages = num_pages;
     P.max_pages = max_pages;
     return ts_rope_run(&P, stream);
+}
+
+/* What the 4-bit pools ask of every call over them. */
+static int ts_kv4_pools_ok(const uint8_t *kc, const uint8_t *ks, const uint8_t *vc, const uint8_t *vs, const int *table,
+                           int D, int page_size, int num_pages, int max_pages) {
+    if (!kc || !ks || !vc || !vs || !table || (D != 64 && D != 128) || num_pages < 1 || max_pages < 1)
+        return ATTN_ERR_ARGS;
+    if (!(page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 ||
+          (page_size > 0 && page_size % 128 == 0)))
+        return ATTN_ERR_ARGS;
+    if ((long long)page_size * max_pages > INT_MAX - 1024) return ATTN_ERR_ARGS;
+    if (!ts_al16(kc) || !ts_al16(ks) || !ts_al16(vc) || !ts_al16(vs)) return ATTN_ERR_ALIGN;
+    return ATTN_OK;
+}
+
+int attn_qkv_rope_kv4_stream(const uint16_t *qkv, const int *positions, const float *cos_sin, int max_pos,
+                             const uint16_t *q_norm_w, const uint16_t *k_norm_w, float eps, int B, int S, int Hq,
+                             int Hkv, int D, int rot, int style, uint16_t *Q, uint8_t *K_codes, uint8_t *K_scales,
+                             uint8_t *V_codes, uint8_t *V_scales, const int *block_table, int page_size, int num_pages,
+                             int max_pages, void *scratch, void *stream) {
+    ts_rope_problem P;
+    int rc = ts_kv4_pools_ok(K_codes, K_scales, V_codes, V_scales, block_table, D, page_size, num_pages, max_pages);
+    if (rc == ATTN_ERR_ARGS) return rc;
+    /* (the pools stand in for the bf16 caches in the shared checks) */
+    const int frc = ts_rope_fill(&P, qkv, positions, cos_sin, max_pos, q_norm_w, k_norm_w, eps, B, S, Hq, Hkv, D, rot,
+                                 style, Q, (uint16_t *)K_codes, (uint16_t *)V_codes, scratch);
+    if (frc != ATTN_OK) return frc;
+    if (rc != ATTN_OK) return rc;
+    P.K = P.V = NULL;
+    P.k_codes = K_codes;
+    P.k_scales = K_scales;
+    P.v_codes = V_codes;
+    P.v_scales = V_scales;
+    P.block_table = block_table;
+    P.page_size = page_size;
+    P.num_pages = num_pages;
+    P.max_pages = max_pages;
+    return ts_rope_run(&P, stream);
+}
+
+int attn_kv4_unpack_stream(const uint8_t *K_codes, const uint8_t *K_scales, const uint8_t *V_codes,
+                           const uint8_t *V_scales, const int *block_table, const int *positions, uint16_t *K,
+                           uint16_t *V, int B, int S, int Hkv, int D, int page_size, int num_pages, int max_pages,
+                           void *scratch, void *stream) {
+    int rc = ts_kv4_pools_ok(K_codes, K_scales, V_codes, V_scales, block_table, D, page_size, num_pages, max_pages);
+    if (rc == ATTN_ERR_ARGS || !positions || !K || !V || !scratch || B < 0 || S < 0 || Hkv < 1) return ATTN_ERR_ARGS;
+    if ((long long)B * S > INT_MAX || (long long)B * Hkv > INT_MAX) return ATTN_ERR_ARGS;
+    if (rc != ATTN_OK || !ts_al16(K) || !ts_al16(V) || ((uintptr_t)scratch % ATTN_SCRATCH_ALIGN) != 0)
+        return ATTN_ERR_ALIGN;
+    if (ts_cc_major() != 10) return ATTN_ERR_NOT_SM100;
+    ts_kv4_problem P;
+    memset(&P, 0, sizeof P);
+    P.k_codes = K_codes;
+    P.k_scales = K_scales;
+    P.v_codes = V_codes;
+    P.v_scales = V_scales;
+    P.block_table = block_table;
+    P.positions = positions;
+    P.K = K;
+    P.V = V;
+    P.B = B;
+    P.S = S;
+    P.Hkv = Hkv;
+    P.D = D;
+    P.page_size = page_size;
+    P.num_pages = num_pages;
+    P.max_pages = max_pages;
+    P.status = (int *)scratch;
+    rc = ts_clear_status(P.status, stream);
+    if (rc != ATTN_OK) return rc;
+    return ts_launch_kv4_unpack(&P, stream);
 }

@@ -121,9 +121,32 @@ typedef struct ts_rope_problem {
     int B, S, Hq, Hkv, D, rot, style, max_pos;
     int cache_len;                         /* contiguous cache rows per (sequence, kv head) */
     int page_size, num_pages, max_pages;   /* paged cache */
+    /* 4-bit paged cache (attn_kv4.h) instead of K and V, when k_codes is not NULL */
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
 } ts_rope_problem;
 
 int ts_launch_qkv_rope(const ts_rope_problem *p, void *stream);
+
+/* The 4-bit cache (attn_kv4.h): its tokens as bf16 (kv4_cache.cu), and attention over it
+ * (kv4_attn.cu). */
+typedef struct ts_kv4_problem {
+    const uint16_t *Q;
+    const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *block_table, *seq_lens, *positions;
+    void *O;                   /* attention output */
+    uint16_t *K, *V;           /* unpacked tokens [B*Hkv][S][D] */
+    int o_bf16, B, S, Hq, Hkv, Sq, D, causal;
+    int page_size, num_pages, max_pages;
+    float scale_log2, cap_in, cap_out;
+    const float *slopes;
+    const int *key_begin, *key_end;
+    int *status;
+    float *part_m, *part_l, *part_acc; /* scratch partial rows */
+    int part_rows;
+} ts_kv4_problem;
+
+int ts_launch_kv4(const ts_kv4_problem *p, void *stream);
+int ts_launch_kv4_unpack(const ts_kv4_problem *p, void *stream);
 int ts_launch_rope_table(float *cos_sin, int max_pos, int rot, double theta, void *stream);
 
 /* A fresh nonzero status generation (fa_problem.status_gen), unique within the process. */

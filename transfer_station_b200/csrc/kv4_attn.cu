@@ -1,0 +1,804 @@
+// kv4_attn.cu -- attention over the 4-bit paged key cache (attn_kv4.h), for single tokens and a few new
+// positions per sequence.
+//
+// What bounds it: the cache bytes, D/2 + D/32 per key and per value, read once (68 B at D = 128 against
+// 256 in bf16). At the measured copy rate an SM receives about 24 bytes, 46 elements, per clock, and
+// every element has to become a number for the tensor cores, so the arithmetic per element decides
+// whether the kernel keeps up:
+//   * Dequantisation is two instructions a pair: one LOP3 puts two nibbles under the fp16 exponent of
+//     1024 (1024 + n, or 1024 + 16 n for the high nibble of a byte), one HFMA2 by (s/16, -64.5 s) or
+//     (s/256, -4.5 s) gives (n - 8) s / 16 exactly: s has 4 significant bits, so 64.5 s and 4.5 s fit
+//     fp16's 11, and the product inside the FMA is not rounded. The factor 16 goes into the score's
+//     scale and the output's. fp16 rather than bf16: the weights P keep 11 bits, and Q, 8 bits wide, is
+//     exact after a power-of-two scale per row.
+//   * Keys are the M side of mma.m16n8k16 and the queries of a kv head the N side, so a group of up to 8
+//     query rows costs one MMA per 16 keys x 16 elements with no padding rows; P^T for the second product
+//     comes from the score fragment by two movmatrix transposes. tcgen05 would need the dequantised tile
+//     written to shared memory (2 bytes an element: 92 of the 128 bytes a clock) and 128 rows of queries
+//     or a TMEM round trip of the weights; here the elements never leave registers.
+//   * A lane's elements of a key are one contiguous run (D/4 of K, D/8 of V), so each key row is read from
+//     shared memory with one vector load a lane, and the k order inside the MMA is whatever the nibbles
+//     give: Q's fragments are permuted to match.
+//
+// Work split. Tiles of kTile keys of all (sequence, kv head, row block) units form one list; CTA c of G
+// takes the c-th G-th of it, whatever the lengths are, so a ragged batch stays balanced without the host
+// knowing a length. A unit cut between CTAs leaves (m, l, acc) partials, merged by kv4_combine.
+// One producer warp per CTA streams tiles into a ring of shared-memory stages with untiled bulk copies;
+// four consumer warps take 16 keys of each tile, each with its own running maximum and accumulator, merged
+// in shared memory at a unit's end.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "attn_kv4.h"
+#include "fa_launch.h"
+#include "score_cap.cuh"
+#include "sm100_ptx.cuh"
+
+extern "C" void ts_count_launch(void);
+
+namespace ts {
+
+namespace {
+
+constexpr int kTile = 64;        // keys per stage
+constexpr int kWarps = 4;        // consumer warps, 16 keys of a tile each
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kMinTiles = 2;     // a CTA takes at least this many tiles (fewer CTAs work on small problems)
+
+constexpr float kHead = 7.f, kMost = 15.f;  // see the weights
+
+struct Kv4Params {
+    const uint16_t *Q;
+    const uint8_t *kc, *ks, *vc, *vs;
+    const int *block_table, *seq_lens;
+    void *O;
+    int o_bf16;
+    int B, Hq, Hkv, Sq, group, row_blocks, causal;
+    int page_size, num_pages, max_pages;
+    float scale_log2;  // log2(e) / sqrt(D)
+    float cap_in, cap_out;
+    const float *slopes;
+    const int *key_begin, *key_end;
+    int *status;                  // [0]: result; [2], [3]: reports of the running call and its generation
+    unsigned gen;
+    float *part_m, *part_l, *part_acc;  // [2 * CTAs][rows]([D]): slot 2c of CTA c for a unit begun before it, 2c + 1 after
+    int2 *desc;                   // [units]: first and last CTA of a unit (equal: nothing to merge)
+};
+
+template <int D, int NT>
+struct Kv4Config {
+    static constexpr int CODES = kTile * D / 2, SCALES = kTile * D / ATTN_KV4_GROUP;
+    static constexpr int STAGE = 2 * (CODES + SCALES);
+    static constexpr int NS = D == 128 ? 5 : 8;
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int MERGE = kWarps * ROWS * (D + 4) * 4;  // one warp's accumulator rows, padded
+    static constexpr int OFF_MERGE = NS * STAGE;
+    static constexpr int OFF_ML = OFF_MERGE + MERGE;           // m, l [kWarps][ROWS]
+    static constexpr int OFF_BAR = OFF_ML + 2 * kWarps * ROWS * 4;
+    static constexpr int SMEM = OFF_BAR + 2 * NS * 8;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+
+// Two E4M3 bytes -> fp16.
+__device__ __forceinline__ __half2 scales2(uint32_t lo, uint32_t hi) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(lo | (hi << 8)), __NV_E4M3);
+    return __half2(r);
+}
+
+// What turns the nibbles of a pair of scales into numbers: see the file's head.
+struct Dequant {
+    __half2 lo, lo_add, hi, hi_add;
+    __device__ __forceinline__ explicit Dequant(__half2 s)
+        : lo(__hmul2(s, __float2half2_rn(1.f / 16.f))),
+          lo_add(__hmul2(s, __float2half2_rn(-64.5f))),
+          hi(__hmul2(s, __float2half2_rn(1.f / 256.f))),
+          hi_add(__hmul2(s, __float2half2_rn(-4.5f))) {}
+    // nibbles at bits 0 and 16, and at bits 4 and 20
+    __device__ __forceinline__ uint32_t low(uint32_t x) const {
+        return as_u32(__hfma2(as_half2((x & 0x000f000fu) | 0x64006400u), lo, lo_add));
+    }
+    __device__ __forceinline__ uint32_t high(uint32_t x) const {
+        return as_u32(__hfma2(as_half2((x & 0x00f000f0u) | 0x64006400u), hi, hi_add));
+    }
+};
+
+// A sequence: its keys, the span [lo, hi) outside which no query of it sees one, and the tiles of that
+// span (at least one, so that a sequence without keys gets its zero rows). The span is read from the key
+// ranges for up to kSpanRows query positions; longer calls walk the whole sequence.
+constexpr int kSpanRows = 16;
+struct Span {
+    int len, lo, hi, t0, nt;
+};
+__device__ __forceinline__ Span seq_span(const Kv4Params &p, int b) {
+    Span s;
+    const int n = ld_plan(p.seq_lens + b), most = p.max_pages * p.page_size;
+    s.len = n < 0 ? 0 : (n < most ? n : most);
+    s.lo = 0;
+    s.hi = s.len;
+    if ((p.key_begin || p.key_end) && p.Sq <= kSpanRows) {
+        int lo = s.len, hi = 0;
+        for (int i = 0; i < p.Sq; ++i) {
+            const size_t at = (size_t)b * p.Sq + i;
+            lo = min(lo, p.key_begin ? ld_plan(p.key_begin + at) : 0);
+            hi = max(hi, p.key_end ? ld_plan(p.key_end + at) : s.len);
+        }
+        s.lo = max(lo, 0);
+        s.hi = min(hi, s.len);
+    }
+    s.t0 = s.lo / kTile;
+    s.nt = s.hi > s.lo ? (s.hi + kTile - 1) / kTile - s.t0 : 1;
+    return s;
+}
+
+// Where a CTA's share of the tile list begins, and what the list is.
+struct Share {
+    long long total, t0, t1;  // all tiles; this CTA's
+    int ctas;                 // CTAs that have a share
+    int b;                    // first sequence
+    int u;                    // first unit within it
+    int tile;                 // first tile of that unit's span
+};
+
+// All threads of the CTA. Units are ordered by sequence, then kv head, then row block.
+__device__ __forceinline__ Share find_share(const Kv4Params &p, int cta, int grid) {
+    __shared__ long long warp_sum[32];
+    __shared__ long long found_rem;
+    __shared__ int found_b;
+    const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = n >> 5;
+    const int units = p.Hkv * p.row_blocks;
+    const int chunk = (p.B + n - 1) / n;
+    const int b0 = min(p.B, tid * chunk), b1 = min(p.B, b0 + chunk);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (long long)seq_span(p, b).nt * units;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    if (tid == 0) found_b = p.B;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    Share s;
+    s.total = total;
+    const long long most = (total + kMinTiles - 1) / kMinTiles;
+    s.ctas = (int)(most < grid ? most : grid);
+    s.t0 = cta < s.ctas ? cta * total / s.ctas : total;
+    s.t1 = cta < s.ctas ? (cta + 1) * total / s.ctas : total;
+    long long at = before + incl - mine;
+    if (s.t0 >= at && s.t0 < at + mine) {
+        int b = b0;
+        for (; b < b1; ++b) {
+            const long long here = (long long)seq_span(p, b).nt * units;
+            if (s.t0 < at + here) break;
+            at += here;
+        }
+        found_b = b;
+        found_rem = s.t0 - at;
+    }
+    __syncthreads();
+    s.b = found_b;
+    s.u = s.tile = 0;
+    if (s.t0 < s.t1) {
+        const int nt = seq_span(p, s.b).nt;
+        s.u = (int)(found_rem / nt);
+        s.tile = (int)(found_rem - (long long)s.u * nt);
+    }
+    return s;
+}
+
+// The CTA that has tile x of the list.
+__device__ __forceinline__ int owner(long long x, long long total, int ctas) {
+    int c = (int)(x * ctas / total);
+    while (c + 1 < ctas && (c + 1) * total / ctas <= x) ++c;
+    return c;
+}
+
+// Reports gather in a pair (generation, codes) that kv4_combine moves to the status word: a report can
+// neither meet the clearing of an earlier call's nor be lost by a replayed graph's.
+__device__ __forceinline__ void report_pending(const Kv4Params &p, int code) {
+    unsigned long long *at = reinterpret_cast<unsigned long long *>(p.status + 2);
+    unsigned long long old = *reinterpret_cast<volatile unsigned long long *>(at);
+    while (true) {
+        const unsigned long long now = (unsigned)(old >> 32) == p.gen ? old | (unsigned)code
+                                                                      : ((unsigned long long)p.gen << 32) | (unsigned)code;
+        const unsigned long long seen = atomicCAS(at, old, now);
+        if (seen == old) return;
+        old = seen;
+    }
+}
+
+// Bounded wait on a barrier of this CTA.
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, const Kv4Params &p,
+                                          int code) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1;
+            report_pending(p, code);
+            return false;
+        }
+    }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv4Params p) {
+    using C = Kv4Config<D, NT>;
+    constexpr int KW = D / 32;             // 32-bit words of a key row that a lane holds (its quarter of the row)
+    constexpr int VW = D / 64;             // words of a value row that a lane holds (its eighth)
+    constexpr int MT = D / 16;             // 16-element tiles of the output
+    constexpr int GROUPS = D / ATTN_KV4_GROUP;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int abort_flag_s;
+    volatile int *abort_flag = &abort_flag_s;
+    const uint32_t base = smem_u32(smem), bars = base + C::OFF_BAR;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (C::NS + s); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        abort_flag_s = 0;
+        for (int s = 0; s < C::NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kWarps);
+        }
+        fence_mbar_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    const Share sh = find_share(p, blockIdx.x, gridDim.x);  // (its barriers also publish the set-up)
+    if (sh.t0 >= sh.t1) return;
+
+    const int units = p.Hkv * p.row_blocks;
+    long long left = sh.t1 - sh.t0;
+    int b = sh.b, u = sh.u, tile = sh.tile;
+
+    if (warp == kWarps) {
+        // ================= producer: the CTA's tiles, in order, into the ring
+        const int P = p.page_size;
+        const int rows = P < kTile ? P : kTile;      // keys per copy
+        const int per_tile = kTile / rows;           // copies per pool and tile
+        long long k = 0;                             // tiles issued
+        bool ok = true;
+        while (left > 0 && ok) {
+            const Span sp = seq_span(p, b);
+            const int len = sp.len, nt = sp.nt;
+            const int kvh = u / p.row_blocks;
+            const int used = (len + P - 1) / P;
+            const int *table = p.block_table + (size_t)b * p.max_pages;
+            const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
+            // chunk ids (a chunk: `rows` keys) of the next 32 chunks, one a lane
+            int win = -1, id = -1;
+            for (int i = tile; i < end && ok; ++i, ++k) {
+                const int c0 = (sp.t0 + i) * per_tile;
+                if (win < 0 || c0 + per_tile > win + 32) {
+                    win = c0;
+                    const long long key = (long long)(c0 + lane) * rows;
+                    const int page = (int)(key / P);
+                    id = -1;
+                    if (key < len && page < used) {
+                        id = ld_plan(table + page);
+                        if (id < 0 || id >= p.num_pages) {
+                            report_pending(p, kDevErrBadPage);
+                            id = -1;
+                        }
+                    }
+                }
+                const int st = (int)(k % C::NS);
+                const uint32_t round = (uint32_t)(k / C::NS);
+                if (round > 0) ok = ring_wait(empty(st), (round - 1) & 1u, abort_flag, p, kDevErrTimeoutKV);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int my_id = __shfl_sync(0xffffffffu, id, (c0 - win + lane) & 31);
+                const bool mine = lane < per_tile && my_id >= 0;
+                const int n = __popc(__ballot_sync(0xffffffffu, mine));
+                const uint32_t code_bytes = (uint32_t)(rows * (D / 2)), scale_bytes = (uint32_t)(rows * GROUPS);
+                if (lane == 0) mbar_expect_tx(full(st), (uint32_t)n * 2u * (code_bytes + scale_bytes));
+                __syncwarp();
+                if (mine) {
+                    const int row0 = (int)(((long long)(c0 + lane) * rows) % P);
+                    const size_t at = ((size_t)my_id * p.Hkv + kvh) * P + row0;  // row of the pools
+                    const uint32_t dst = base + st * C::STAGE, bar = full(st);
+                    bulk_load(dst + lane * code_bytes, p.kc + at * (D / 2), code_bytes, bar);
+                    bulk_load(dst + C::CODES + lane * scale_bytes, p.ks + at * GROUPS, scale_bytes, bar);
+                    bulk_load(dst + C::CODES + C::SCALES + lane * code_bytes, p.vc + at * (D / 2), code_bytes, bar);
+                    bulk_load(dst + 2 * C::CODES + C::SCALES + lane * scale_bytes, p.vs + at * GROUPS, scale_bytes, bar);
+                }
+                __syncwarp();
+            }
+            left -= end - tile;
+            tile = 0;
+            if (++u == units) {
+                u = 0;
+                ++b;
+            }
+        }
+        // copies in flight land before the CTA exits: the last issue of each stage
+        for (long long j = k > C::NS ? k - C::NS : 0; j < k; ++j) {
+            volatile int never = 0;
+            ring_wait(full((int)(j % C::NS)), (uint32_t)(j / C::NS) & 1u, &never, p, kDevErrTimeoutDrain);
+        }
+        return;
+    }
+
+    // ================= consumers
+    const int g = lane >> 2, t = lane & 3;
+    float *merge = reinterpret_cast<float *>(smem + C::OFF_MERGE);
+    float *ml = reinterpret_cast<float *>(smem + C::OFF_ML);
+    const int rows_all = p.group * p.Sq;
+    const bool has_cap = p.cap_out > 0.f, has_bias = p.slopes != nullptr;
+    long long k = 0;
+    bool ok = true;
+    while (left > 0) {
+        const Span span = seq_span(p, b);
+        const int len = span.len, nt = span.nt;
+        const int kvh = u / p.row_blocks, rb = u - kvh * p.row_blocks;
+        const int begin = tile, end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
+        const int row0 = rb * C::ROWS;
+        const size_t qrow0 = ((size_t)b * p.Hkv + kvh) * rows_all + row0;  // row of Q and O
+
+        // ---- Q fragments: lane (g, t) holds query row g's quarter t, scaled by a power of two per row
+        uint32_t qf[NT][D / 16][2];
+        float fac[NT][2];  // raw score -> scaled score, for this lane's two query columns
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const bool have = row0 + 8 * n + g < rows_all;
+            const uint16_t *src = p.Q + (qrow0 + 8 * n + g) * D + t * (D / 4);
+            uint32_t raw[D / 8];
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (have) v = *reinterpret_cast<const uint4 *>(src + 8 * w);
+                raw[4 * w] = v.x, raw[4 * w + 1] = v.y, raw[4 * w + 2] = v.z, raw[4 * w + 3] = v.w;
+            }
+            float a = 0.f;
+#pragma unroll
+            for (int w = 0; w < D / 8; ++w)
+                a = fmaxf(a, fmaxf(fabsf(__uint_as_float(raw[w] << 16)), fabsf(__uint_as_float(raw[w] & 0xffff0000u))));
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+            // 2^-e with the row's largest magnitude in [1, 2) after it (a zero or non-finite row stays)
+            const int e = (int)(__float_as_uint(a) >> 23) - 127;
+            const bool plain = a == 0.f || e >= 128 || e <= -126;
+            const float down = plain ? 1.f : __uint_as_float((uint32_t)(127 - e) << 23);
+            const float up = plain ? 1.f : __uint_as_float((uint32_t)(127 + e) << 23);
+            // word w of a key row holds nibbles 0..7 = elements 8w..8w+7 in pairs (0,4) (1,5) (2,6) (3,7)
+            auto element = [&](int i) {
+                const uint32_t v = raw[i >> 1];
+                return __uint_as_float((i & 1) ? (v & 0xffff0000u) : (v << 16)) * down;
+            };
+#pragma unroll
+            for (int w = 0; w < KW; ++w)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    qf[n][2 * w + (h >> 1)][h & 1] =
+                        as_u32(__floats2half2_rn(element(8 * w + h), element(8 * w + h + 4)));
+            const float c0 = __shfl_sync(0xffffffffu, up, 8 * t), c1 = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+            const float unit = 16.f * (has_cap ? p.cap_in : p.scale_log2);
+            fac[n][0] = c0 * unit;
+            fac[n][1] = c1 * unit;
+        }
+        // ---- this lane's query columns: keys seen, position, bias
+        int lo[NT][2], hi[NT][2], pos[NT][2], near[NT][2];
+        float slope2[NT][2];
+        int all_lo = 0, all_hi = len;  // every row sees [all_lo, all_hi)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int row = min(row0 + 8 * n + 2 * t + c, rows_all - 1), i = row % p.Sq;
+                pos[n][c] = len - p.Sq + i;
+                lo[n][c] = 0;
+                hi[n][c] = p.causal ? min(len, pos[n][c] + 1) : len;
+                const size_t at = (size_t)b * p.Sq + i;
+                if (p.key_begin) lo[n][c] = min(max(0, ld_plan(p.key_begin + at)), len);
+                if (p.key_end) hi[n][c] = min(hi[n][c], ld_plan(p.key_end + at));
+                hi[n][c] = max(hi[n][c], 0);
+                near[n][c] = max(0, max(lo[n][c] - pos[n][c], pos[n][c] - (hi[n][c] - 1)));
+                slope2[n][c] = has_bias ? ld_plan(p.slopes + kvh * p.group + row / p.Sq) * 1.4426950408889634f : 0.f;
+                all_lo = max(all_lo, lo[n][c]);
+                all_hi = min(all_hi, hi[n][c]);
+            }
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+
+        float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[n][i][c] = 0.f;
+        }
+
+        for (int i = begin; i < end; ++i, ++k) {
+            const int st = (int)(k % C::NS);
+            if (ok) ok = ring_wait(full(st), (uint32_t)(k / C::NS) & 1u, abort_flag, p, kDevErrTimeoutKV);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint8_t *stage = smem + st * C::STAGE;
+            const int key0 = (span.t0 + i) * kTile + 16 * warp;            // this warp's 16 keys
+            const bool edge = key0 < span.lo || key0 + 16 > span.hi;       // some are not the sequence's to see
+            // ---- S^T = K Q^T
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            {
+                const int r0 = 16 * warp + g;
+                const uint8_t *rowp = stage + r0 * (D / 2) + t * (D / 8);
+                uint32_t ka[KW], kb[KW];
+                if constexpr (KW == 4) {
+                    *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(rowp);
+                    *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(rowp + 8 * (D / 2));
+                } else {
+                    *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(rowp);
+                    *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(rowp + 8 * (D / 2));
+                }
+                const uint8_t *sp = stage + C::CODES + r0 * GROUPS + t * GROUPS / 4;
+                const uint32_t sa = sp[0], sb = sp[8 * GROUPS];
+                const Dequant da(scales2(sa, sa)), db(scales2(sb, sb));
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    uint32_t x = ka[w], y = kb[w];
+                    uint32_t a[4] = {da.low(x), db.low(y), da.high(x), db.high(y)};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(s[n], a, qf[n][2 * w][0], qf[n][2 * w][1]);
+                    x >>= 8;
+                    y >>= 8;
+                    a[0] = da.low(x), a[1] = db.low(y), a[2] = da.high(x), a[3] = db.high(y);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(s[n], a, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                }
+            }
+            // ---- scores in log2 units: element e of s is key g + 8 (e / 2), query column e % 2
+            const bool whole = key0 >= all_lo && key0 + 16 <= all_hi;
+            bool above = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = e & 1;
+                    float z = s[n][e] * fac[n][c];
+                    if (has_cap) z = cap_exact(z, p.cap_out);
+                    const int key = key0 + g + 8 * (e >> 1);
+                    if (has_bias) z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
+                    if (!whole && (key < lo[n][c] || key >= hi[n][c])) z = -INFINITY;
+                    s[n][e] = z;
+                    above |= z > m[n][c] + kMost;
+                }
+            // A column's reference m is its maximum less kHead when it was set, and moves only when a score
+            // exceeds m + kMost. Weights 2^(z - m) thus reach from 2^kHead at the maximum up to 2^kMost,
+            // inside fp16's range, and keep 11 bits down to 2^-(14 + kHead) of the largest; below that the
+            // step is 2^-(24 + kHead) of it.
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = fmaxf(s[n][c], s[n][c + 2]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float to = fmaxf(m[n][c], mx - kHead);
+                        const float alpha = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - to);
+                        m[n][c] = to;
+                        l[n][c] *= alpha;
+#pragma unroll
+                        for (int q = 0; q < MT; ++q) {
+                            acc[n][q][c] *= alpha;
+                            acc[n][q][c + 2] *= alpha;
+                        }
+                    }
+            }
+            // ---- weights, and their transpose as the B operand of O^T += V^T P^T
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mm = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1];
+                    w[e] = ex2(s[n][e] - mm);
+                    l[n][e & 1] += w[e];
+                }
+                pf[n][0] = transpose8x8(as_u32(__floats2half2_rn(w[0], w[1])));
+                pf[n][1] = transpose8x8(as_u32(__floats2half2_rn(w[2], w[3])));
+            }
+            // ---- V^T: rows are this lane's D/8 elements, columns keys 2t, 2t+1, 2t+8, 2t+9
+            {
+                const uint8_t *vp = stage + C::CODES + C::SCALES + (16 * warp + 2 * t) * (D / 2) + g * (D / 16);
+                const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + (16 * warp + 2 * t) * GROUPS + g * GROUPS / 8;
+                uint32_t v[4][VW];
+                uint32_t sc[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = (j & 1) + 8 * (j >> 1);
+                    if constexpr (VW == 2)
+                        *reinterpret_cast<uint2 *>(v[j]) = *reinterpret_cast<const uint2 *>(vp + r * (D / 2));
+                    else
+                        v[j][0] = *reinterpret_cast<const uint32_t *>(vp + r * (D / 2));
+                    sc[j] = sp[r * GROUPS];
+                    // what an unseen slot holds may be any byte, a NaN scale among them: it becomes zero
+                    if (edge && (key0 + 2 * t + r < span.lo || key0 + 2 * t + r >= span.hi)) sc[j] = 0u;
+                }
+                const Dequant d0(scales2(sc[0], sc[1])), d1(scales2(sc[2], sc[3]));
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        // the same half word of both keys: nibble n of each half is element 8w + 4h + n
+                        uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
+                        uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+                        uint32_t a[4] = {d0.low(x), d0.high(x), d1.low(y), d1.high(y)};
+                        const int i0 = 4 * w + 2 * h;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816(acc[n][i0], a, pf[n][0], pf[n][1]);
+                        x >>= 8;
+                        y >>= 8;
+                        a[0] = d0.low(x), a[1] = d0.high(x), a[2] = d1.low(y), a[3] = d1.high(y);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816(acc[n][i0 + 1], a, pf[n][0], pf[n][1]);
+                    }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(st));
+        }
+
+        // ---- merge the four warps: rows [ROWS] x D
+        // lane (g, t) holds, for query columns 2t and 2t+1, the D/8 consecutive elements from g * D/8
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
+                l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
+                l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
+                if (g == 0) {
+                    ml[warp * C::ROWS + 8 * n + 2 * t + c] = m[n][c];
+                    ml[(kWarps + warp) * C::ROWS + 8 * n + 2 * t + c] = l[n][c];
+                }
+                float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (D + 4) + g * (D / 8);
+#pragma unroll
+                for (int i = 0; i < MT; i += 2)
+                    *reinterpret_cast<float4 *>(dst + 2 * i) = make_float4(acc[n][i][c], acc[n][i][c + 2],
+                                                                          acc[n][i + 1][c], acc[n][i + 1][c + 2]);
+            }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+        const bool cut = begin > 0 || end < nt;
+        const size_t slot = ((size_t)2 * blockIdx.x + (begin > 0 ? 0 : 1)) * C::ROWS;
+        if (threadIdx.x == 0 && begin == 0) {
+            int2 d = make_int2(blockIdx.x, blockIdx.x);
+            if (cut) {  // the unit's last tile: this CTA's share ends inside the unit
+                const long long at = sh.t1 - left + nt - 1;
+                d.y = owner(at, sh.total, sh.ctas);
+            }
+            p.desc[(size_t)b * units + u] = d;
+        }
+        constexpr int V4 = D / 4;
+        for (int x = threadIdx.x; x < C::ROWS * V4; x += 32 * kWarps) {
+            const int r = x / V4, c4 = x - r * V4;
+            float mw[kWarps], M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                mw[w] = ml[w * C::ROWS + r];
+                M = fmaxf(M, mw[w]);
+            }
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
+                const float4 v = *reinterpret_cast<const float4 *>(merge + (w * C::ROWS + r) * (D + 4) + 4 * c4);
+                L = fmaf(f, ml[(kWarps + w) * C::ROWS + r], L);
+                o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+            }
+            if (cut) {
+                if (c4 == 0) {
+                    p.part_m[slot + r] = M;
+                    p.part_l[slot + r] = L;
+                }
+                *reinterpret_cast<float4 *>(p.part_acc + (slot + r) * D + 4 * c4) = o;
+            } else if (row0 + r < rows_all) {
+                // V carries s/16
+                const float inv = L > 0.f ? 16.f / L : (L == 0.f ? 0.f : L);
+                const size_t at = (qrow0 + r) * D + 4 * c4;
+                if (p.o_bf16)
+                    *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.O) + at) =
+                        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                else
+                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.O) + at) =
+                        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");  // the merge area is free again
+        left -= end - begin;
+        tile = 0;
+        if (++u == units) {
+            u = 0;
+            ++b;
+        }
+    }
+}
+
+// Merges a cut unit's partials: block (unit, row), its warps take pieces in turn. Block 0 also moves the
+// call's reports to the status word.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv4_combine(const Kv4Params p) {
+    constexpr int ROWS = 8 * NT, PER = D / 32;
+    __shared__ float sm[4], sl[4], sacc[4][D];
+    pdl_wait();
+    pdl_trigger();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+        unsigned long long *at = reinterpret_cast<unsigned long long *>(p.status + 2);
+        const unsigned long long v = *reinterpret_cast<volatile unsigned long long *>(at);
+        p.status[0] = (unsigned)(v >> 32) == p.gen ? (int)(unsigned)v : 0;
+        *at = 0;
+    }
+    const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int units = p.Hkv * p.row_blocks;
+    const int2 d = make_int2(ld_plan(&p.desc[blockIdx.x].x), ld_plan(&p.desc[blockIdx.x].y));
+    if (d.x == d.y) return;
+    const int b = blockIdx.x / units, u = blockIdx.x - b * units;
+    const int kvh = u / p.row_blocks, rb = u - kvh * p.row_blocks;
+    const int row = rb * ROWS + r, rows_all = p.group * p.Sq;
+    if (row >= rows_all) return;
+    auto slot = [&](int c) { return ((size_t)2 * c + (c == d.x ? 1 : 0)) * ROWS + r; };
+    float m = -INFINITY, l = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    for (int c = d.x + warp; c <= d.y; c += 4) {
+        const size_t at = slot(c);
+        const float mc = p.part_m[at], lc = p.part_l[at];
+        float v[PER];
+        if constexpr (PER == 4) {
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p.part_acc + at * D + PER * lane);
+        } else {
+            *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p.part_acc + at * D + PER * lane);
+        }
+        const float to = fmaxf(m, mc);
+        const float f0 = m == -INFINITY ? 0.f : ex2(m - to), f1 = mc == -INFINITY ? 0.f : ex2(mc - to);
+        l = l * f0 + lc * f1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = acc[i] * f0 + v[i] * f1;
+        m = to;
+    }
+    if (lane == 0) {
+        sm[warp] = m;
+        sl[warp] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sacc[warp][PER * lane + i] = acc[i];
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col >= D) return;
+    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - M);
+        L = fmaf(f, sl[w], L);
+        o = fmaf(f, sacc[w][col], o);
+    }
+    const float inv = L > 0.f ? 16.f / L : (L == 0.f ? 0.f : L);
+    const size_t at = (((size_t)b * p.Hkv + kvh) * rows_all + row) * D + col;
+    if (p.o_bf16)
+        reinterpret_cast<uint16_t *>(p.O)[at] = (uint16_t)pack_bf16x2(o * inv, 0.f);
+    else
+        reinterpret_cast<float *>(p.O)[at] = o * inv;
+}
+
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return ATTN_ERR_CUDA;
+    ts_count_launch();
+    return ATTN_OK;
+}
+
+// CTAs of this kernel that fit on an SM (cached per device, with the shared-memory opt-in done).
+template <int D, int NT>
+int resident() {
+    static std::atomic<int> cache[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return -1;
+    const bool cached = dev >= 0 && dev < 64;
+    if (cached) {
+        const int r = cache[dev].load(std::memory_order_acquire);
+        if (r > 0) return r;
+    }
+    auto kern = kv4_kernel<D, NT>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv4Config<D, NT>::SMEM) != cudaSuccess)
+        return -1;
+    int r = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r, kern, kThreads, Kv4Config<D, NT>::SMEM) != cudaSuccess || r < 1)
+        r = 1;
+    if (cached) cache[dev].store(r, std::memory_order_release);
+    return r;
+}
+
+template <int D, int NT>
+int run(const ts_kv4_problem *P, cudaStream_t st) {
+    const int fit = resident<D, NT>();
+    if (fit < 0) return ATTN_ERR_CUDA;
+    Kv4Params p;
+    p.Q = P->Q;
+    p.kc = P->k_codes, p.ks = P->k_scales, p.vc = P->v_codes, p.vs = P->v_scales;
+    p.block_table = P->block_table;
+    p.seq_lens = P->seq_lens;
+    p.O = P->O;
+    p.o_bf16 = P->o_bf16;
+    p.B = P->B, p.Hq = P->Hq, p.Hkv = P->Hkv, p.Sq = P->Sq;
+    p.group = P->Hq / P->Hkv;
+    p.row_blocks = (p.group * P->Sq + 8 * NT - 1) / (8 * NT);
+    p.causal = P->causal;
+    p.page_size = P->page_size, p.num_pages = P->num_pages, p.max_pages = P->max_pages;
+    p.scale_log2 = P->scale_log2;
+    p.cap_in = P->cap_in, p.cap_out = P->cap_out;
+    p.slopes = P->slopes;
+    p.key_begin = P->key_begin, p.key_end = P->key_end;
+    p.status = P->status;
+    p.gen = ts_next_status_gen();
+    const long long units = (long long)P->B * P->Hkv * p.row_blocks;
+    const long long tiles = ((long long)P->max_pages * P->page_size + kTile - 1) / kTile;
+    long long ctas = (long long)ts_num_sms() * fit;
+    if (ctas > P->part_rows / (2 * 8 * NT)) ctas = P->part_rows / (2 * 8 * NT);
+    if (tiles * units < ctas) ctas = tiles * units;
+    // the partials: rows of the first 2 * ctas slots; the units' descriptors behind their accumulators
+    p.part_m = P->part_m;
+    p.part_l = P->part_l;
+    p.part_acc = P->part_acc;
+    const size_t acc = (size_t)2 * ctas * 8 * NT * D;
+    if (acc * 4 + (size_t)units * sizeof(int2) > (size_t)P->part_rows * D * 4) return ATTN_ERR_ARGS;
+    p.desc = reinterpret_cast<int2 *>(P->part_acc + acc);
+    const int rc = launch(kv4_kernel<D, NT>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, p);
+    if (rc != ATTN_OK) return rc;
+    return launch(kv4_combine<D, NT>, dim3((unsigned)units, 8 * NT), dim3(128), 0, st, p);
+}
+
+}  // namespace
+
+}  // namespace ts
+
+extern "C" int ts_launch_kv4(const ts_kv4_problem *P, void *stream) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long rows = (long long)(P->Hq / P->Hkv) * P->Sq;
+    // up to 8 query rows of a kv head: one column tile; more: two, so that a cache row serves 16
+    if (P->D == 64) return rows <= 8 ? ts::run<64, 1>(P, st) : ts::run<64, 2>(P, st);
+    return rows <= 8 ? ts::run<128, 1>(P, st) : ts::run<128, 2>(P, st);
+}
