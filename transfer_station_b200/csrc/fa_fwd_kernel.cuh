@@ -100,6 +100,8 @@ struct TcParams {
     const float *slopes;  // [query heads of one sequence]: distance bias
     float cap_in;         // 1 / (cap * sqrt(D)): raw score -> argument of tanh
     float cap_out;        // cap * log2(e)
+    float cap_ref;        // the fixed reference of capped scores, or negative: a running maximum
+    float tanh_k[6];      // cap_out times the tanh polynomial's coefficients
 };
 
 // What MOD adds to the scores (every MOD != 0 also has the key ranges).
@@ -220,6 +222,14 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         int sk, sk_total;  // keys present (local) and the key axis length the causal rule uses
         int ulo, uhi;      // MOD: no row of the unit sees a key outside [ulo, uhi) ...
         int ilo, ihi;      // ... and every row sees every key of [ilo, ihi)
+        int near;          // MOD with a distance bias: the block the walk begins with
+    };
+    // The item's j-th key block. With a distance bias the walk begins at the unit's own position and goes
+    // back, then ahead: weights fall on the way, where walking from the far end would raise every row's
+    // maximum at every block.
+    auto block_of = [&](const Item &it, int j) {
+        if constexpr (MOD >= kModBias) return j <= it.near ? it.near - j : j;
+        return j;
     };
     auto item_at = [&](int q) {
         Item it;
@@ -311,6 +321,10 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             if (it.ulo > it.kb0) it.kb0 += (it.ulo - it.kb0) / kBN * kBN;
         }
         it.nblk = kend > it.kb0 ? (kend - it.kb0 + kBN - 1) / kBN : 0;
+        if constexpr (MOD >= kModBias) {
+            const int pos = it.sk_total - p.Sq + it.row0 % p.Sq;
+            it.near = p.causal ? it.nblk - 1 : max(0, min((pos - it.kb0) / kBN, it.nblk - 1));
+        }
         return it;
     };
     // this CTA's r-th item (or >= n_items when there is none)
@@ -428,10 +442,11 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             int win_base = -1;
             const int nload = 2 * it.nblk;
             for (int i = 0; i < nload; ++i, ++gl) {
-                const int key0 = kb0 + (i >> 1) * kBN;
+                const int key0 = kb0 + block_of(it, i >> 1) * kBN;
                 const int pg_lo = key0 / P, pg_hi = (key0 + kBN - 1) / P;
-                if (win_base < 0 || pg_hi >= win_base + C::PID_WIN) {  // warp-uniform
+                if (win_base < 0 || pg_hi >= win_base + C::PID_WIN || (MOD >= kModBias && pg_lo < win_base)) {  // warp-uniform
                     win_base = pg_lo;
+                    if (MOD >= kModBias && (i >> 1) <= it.near) win_base = max(0, pg_hi - C::PID_WIN + 1);  // going back
                     bool bad = false;
                     for (int e = lane; e < C::PID_WIN; e += 32) {
                         const int pg = win_base + e;
@@ -526,7 +541,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                         ok = false;
                         break;
                     }
-                    const int key0 = kb0 + (i >> 1) * kBN;
+                    const int key0 = kb0 + block_of(it, i >> 1) * kBN;
                     const uint32_t dst = sKV + slot * C::KVTILE;
                     const uint32_t bar = kv_full(slot);
                     mbar_expect_tx(bar, C::KVTILE);
@@ -672,6 +687,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         const uint32_t tO = tmem_base + lane_off + NQT * kBN + t * DP;
         const float sl2 = p.scale_log2;
         const float2 c2 = make_float2(sl2, sl2);
+        constexpr bool kCap = MOD == kModCap || MOD == kModCapBias, kBias = MOD >= kModBias;
         uint32_t sp = 0;  // score-tile phases consumed, over all items
         uint32_t op = 0;  // items finished (o_full phases consumed)
         uint32_t seen_turn = 0;  // MOD: buffer of the next union of rows' keys
@@ -694,9 +710,8 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         float ms = 0.f;  // m * scale_log2, rounded once (0 while m is -inf)
         // MOD: this row's keys [lo, hi) and its query position; rows past the problem follow the last one.
         int lo = 0, hi = 0, qpos = 0, near = 0;
-        float slope2 = 0.f;  // distance bias per key, log2 units
-        int lo_b = 0, hi_b = 0;   // the keys of the row 128 further on (the unit's other tile)
-        bool far_scores = false;  // capped scores have left the polynomial's interval in this item
+        float slope2 = 0.f;      // distance bias per key, log2 units
+        int lo_b = 0, hi_b = 0;  // the keys of the row 128 further on (the unit's other tile)
         if constexpr (MOD != 0) {
             auto row_keys = [&](int row, int &first, int &end) {
                 const int i = row % p.Sq;
@@ -717,16 +732,16 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 near = max(0, max(lo - qpos, qpos - (hi - 1)));
             }
             hi = min(hi, kb1);  // of this piece
+            if (kCap && p.cap_ref >= 0.f) m = p.cap_ref;
         }
         for (int j = 0; j < nblk; ++j) {
+            if constexpr (MOD == 0) {
             // The path decisions need no scores, so they are made before the wait.
             const long long key0 = kb0 + (long long)j * kBN;
             const long long nv = lastkey - key0 + 1;
             // `full`: every row of this warp sees every key of the block (no tail, no causal
             // cut). The choice must be warp-uniform: every path issues warp-collective tcgen05.st.
-            const int n0 = MOD != 0 ? (int)min(max((long long)lo - key0, 0ll), (long long)kBN) : 0;
-            const int n1 = MOD != 0 ? (int)min(max((long long)hi - key0, 0ll), (long long)kBN) : 0;
-            const bool full = __all_sync(0xffffffffu, MOD != 0 ? (n0 == 0 && n1 == kBN) : nv >= kBN);
+            const bool full = __all_sync(0xffffffffu, nv >= kBN);
             // `spec`: a full block of a warp whose rows all have a running max. P is computed
             // against that max, so the exponentials do not wait for a max pass over all 128
             // columns first. A row whose block max exceeds its running max by more than
@@ -736,10 +751,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             // is tracked. The redo is rare: the first block sets a max that later blocks seldom
             // exceed by that much (a sum above the bound with no single P above it only costs
             // the exact pass).
-            // MOD: a distance bias is linear in the key only on one side of the query position.
-            const bool past = MOD < kModBias || __all_sync(0xffffffffu, key0 + kBN - 1 <= qpos);
-            const bool ahead = MOD >= kModBias && __all_sync(0xffffffffu, key0 >= qpos);
-            const bool spec = full && __all_sync(0xffffffffu, m != -INFINITY) && (past || ahead) && !far_scores;
+            const bool spec = full && __all_sync(0xffffffffu, m != -INFINITY);
             ok = mbar_wait(s_full(t), sp & 1, abort_flag, p.status, kDevErrTimeoutS, p.gen);
             ++sp;
             ok = __all_sync(0xffffffffu, ok);
@@ -748,55 +760,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             uint32_t sr[128];
             float rs0 = 0.f, rs1 = 0.f;
             bool redo = true;
-            if (MOD != 0 && spec) {
-                // As below, on z = the modified score in log2 units (m is a max of z): per pair of
-                // columns z - m = raw * scale + t, or tanh's polynomial in place of the product, with
-                // t = bias - m. A capped score whose argument leaves the polynomial's interval sends
-                // the block to the exact pass, and the later blocks of the item straight there.
-                float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-                const float bs = past ? slope2 : -slope2;
-                const float b0 = MOD >= kModBias ? fmaf(bs, (float)(int)(key0 - (past ? qpos - near : qpos + near)), -m) : -m;
-                const float2 bs2 = make_float2(bs, bs), b02 = make_float2(b0, b0);
-                const float2 in2 = make_float2(p.cap_in, p.cap_in);
-                float far2 = 0.f;
-                tmem_ld16p(tS, sr);
-#pragma unroll
-                for (int cc = 0; cc < 8; ++cc) {
-                    uint32_t pk[8];
-                    if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int c = 16 * cc + 2 * u;
-                        const float2 raw = make_float2(u2f(sr[c]), u2f(sr[c + 1]));
-                        const float2 t = MOD >= kModBias ? __ffma2_rn(make_float2((float)c, (float)(c + 1)), bs2, b02) : b02;
-                        float2 x;
-                        if constexpr (MOD == kModCap || MOD == kModCapBias) {
-                            const float2 y = __fmul2_rn(raw, in2);
-                            const float2 w = __fmul2_rn(y, y);
-                            far2 = fmax3(far2, w.x, w.y);
-                            x = __ffma2_rn(y, tanh_poly(w, p.cap_out), t);
-                        } else {
-                            x = __ffma2_rn(raw, c2, t);
-                        }
-                        float2 pr;
-                        pr.x = ex2(x.x);
-                        pr.y = ex2(x.y);
-                        if (u & 1)
-                            acc1 = __fadd2_rn(acc1, pr);
-                        else
-                            acc0 = __fadd2_rn(acc0, pr);
-                        pk[u] = pack_bf16x2(pr.x, pr.y);
-                    }
-                    tmem_st8(tS + cc * 8, pk);
-                    if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
-                }
-                rs0 = acc0.x + acc1.x;
-                rs1 = acc0.y + acc1.y;
-                // (a NaN leaves the comparisons false; the row is NaN either way)
-                far_scores = __any_sync(0xffffffffu, far2 > kTanhMaxSq);
-                redo = far_scores || __any_sync(0xffffffffu, rs0 + rs1 > kRedoSum);
-                if (redo) tmem_wait_st();  // the speculative P stores land before the exact ones
-            } else if (spec) {
+            if (spec) {
                 const float2 nms2 = make_float2(-ms, -ms);
                 float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
                 // 16 score columns at a time: the next chunk's load is issued before this
@@ -836,7 +800,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 rs1 = acc0.y + acc1.y;
                 redo = __any_sync(0xffffffffu, rs0 + rs1 > kRedoSum);
                 if (redo) tmem_wait_st();  // the speculative P stores land before the exact ones
-            } else if (__all_sync(0xffffffffu, MOD != 0 ? n1 <= n0 : nv <= 0)) {
+            } else if (__all_sync(0xffffffffu, nv <= 0)) {
                 // No row of this warp sees any key of the block (a causal tile below the
                 // diagonal of its item's last block): P = 0, m, l and O stay as they are.
                 uint32_t zero[16];
@@ -852,22 +816,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 l += rs0 + rs1;
             } else {
                 float mb;
-                if constexpr (MOD != 0) {
-                    // every column: modified score in log2 units, -inf outside the row's keys
-                    const float d0 = (float)(int)(key0 - qpos), fnear = (float)near;
-#pragma unroll
-                    for (int c = 0; c < 128; ++c) {
-                        float z;
-                        if constexpr (MOD == kModCap || MOD == kModCapBias)
-                            z = cap_exact(u2f(sr[c]) * p.cap_in, p.cap_out);
-                        else
-                            z = u2f(sr[c]) * sl2;
-                        if constexpr (MOD >= kModBias) z = fmaf(-slope2, fabsf(d0 + (float)c) - fnear, z);
-                        if (!full && (c < n0 || c >= n1)) z = -INFINITY;
-                        sr[c] = f2u(z);
-                    }
-                }
-                if (full || MOD != 0) {
+                if (full) {
                     float mx[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) mx[k] = fmax3(u2f(sr[k]), u2f(sr[8 + k]), u2f(sr[16 + k]));
@@ -893,27 +842,11 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     }
                     mb = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
                 }
-                // MOD keeps m in log2 units, the plain form in units of the raw score
-                const float mu = MOD != 0 ? 1.f : sl2;
                 float m_new = m;
-                if (mb > m && (m == -INFINITY || (mb - m) * mu > kRescaleLog2)) m_new = mb;
-                const float alpha = (m_new == m) ? 1.f : ((m == -INFINITY) ? 0.f : ex2((m - m_new) * mu));
-                ms = (m_new == -INFINITY) ? 0.f : __fmul_rn(m_new, mu);
-                if constexpr (MOD != 0) {
-                    rs0 = rs1 = 0.f;  // a redone block's sums start over
-#pragma unroll
-                    for (int cc = 0; cc < 4; ++cc) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int u = 0; u < 16; ++u) {
-                            const float p0 = ex2(u2f(sr[32 * cc + 2 * u]) - ms), p1 = ex2(u2f(sr[32 * cc + 2 * u + 1]) - ms);
-                            rs0 += p0;
-                            rs1 += p1;
-                            pk[u] = pack_bf16x2(p0, p1);
-                        }
-                        tmem_st16(tS + cc * 16, pk);
-                    }
-                } else if (full) {
+                if (mb > m && (m == -INFINITY || (mb - m) * sl2 > kRescaleLog2)) m_new = mb;
+                const float alpha = (m_new == m) ? 1.f : ((m == -INFINITY) ? 0.f : ex2((m - m_new) * sl2));
+                ms = (m_new == -INFINITY) ? 0.f : __fmul_rn(m_new, sl2);
+                if (full) {
                     // P = 2^(s*c - m*c) by one packed FMA per pair; 3 of every 8 pairs take the
                     // polynomial exp2 on the FMA pipe, the rest the MUFU unit, so both run at once.
                     const float2 nms2 = make_float2(-ms, -ms);
@@ -973,47 +906,245 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     }
                 }
             }
-            if constexpr (MOD != 0) {
-                // V rows that no row of the unit sees (what an unused slot holds, a key between two
-                // ranges) become zero before P V reads them: 0 * NaN would reach every row. PV_0 is
-                // issued first, after every thread of this warpgroup arrived.
-                if (t == 0 && (key0 < it.ilo || key0 + kBN > it.ihi)) {
-                    bool keep = key0 + r >= it.ulo && key0 + r < it.uhi;
-                    if (p.key_begin || p.key_end) {
-                        // the union of both tiles' rows as 128 bits, a word per 32 keys
-                        uint32_t *buf = seen_bits + 16 * (seen_turn & 1);
-                        ++seen_turn;
-                        const int m0 = (int)min(max((long long)lo_b - key0, 0ll), (long long)kBN);
-                        const int m1 = (int)min(max((long long)hi_b - key0, 0ll), (long long)kBN);
+            } else {
+            // Modified scores. z = the modified score in log2 units; m is kept in the same units.
+            //   none     no row of the warp sees a key of the block: P = 0
+            //   fixed    capped scores lie within +-cap_out: up to cap_out = 75 (a cap of 52) the fixed
+            //            reference cap_ref keeps every P in [2^-100, 2^50], so there is no maximum, no
+            //            rescale and no second look -- one pass over the scores
+            //   spec     the plain kernel's speculation: P against the running max, redone when a row
+            //            sum shows a max that moved by more than 2^kRescaleLog2
+            //   general  two passes over the score tile: the max, then P
+            // All but spec are rolled loops of 16 columns: unrolled, the capped form was 60 KB of code
+            // and waited for instructions more than for anything else (2.1 of 9.5 cycles per issue).
+            const int key0 = kb0 + block_of(it, j) * kBN;
+            const int n0 = max(lo - key0, 0), n1 = min(hi - key0, kBN);  // this row's columns [n0, n1)
+            // The choice must be warp-uniform: every path issues warp-collective tcgen05.st.
+            const bool full = __all_sync(0xffffffffu, n0 == 0 && n1 == kBN);
+            const bool none = __all_sync(0xffffffffu, n1 <= n0);
+            // a distance bias is linear in the key on each side of the query position
+            const bool past = !kBias || __all_sync(0xffffffffu, key0 + kBN - 1 <= qpos);
+            const bool ahead = kBias && __all_sync(0xffffffffu, key0 >= qpos);
+            const float bs = past ? slope2 : -slope2;
+            const float b0 = kBias ? bs * (float)(key0 - (past ? qpos - near : qpos + near)) : 0.f;
+            const bool fixed = kCap && p.cap_ref >= 0.f;
+            const bool spec = !kCap && full && (past || ahead) && __all_sync(0xffffffffu, m != -INFINITY);
+            ok = mbar_wait(s_full(t), sp & 1, abort_flag, p.status, kDevErrTimeoutS, p.gen);
+            ++sp;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            // 16 columns from c0: raw scores -> z + add (-inf outside the row's keys)
+            auto scores = [&](const uint32_t *raw, int c0, float add, float2 *z) {
+                const float2 add2 = make_float2(add, add), bs2 = make_float2(bs, bs);
+                const float2 b02 = make_float2(b0 + add, b0 + add);
+                if constexpr (kCap) {
+                    const float2 in2 = make_float2(p.cap_in, p.cap_in);
+                    float far = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t w = span_bits(n0 - 32 * k, n1 - 32 * k) |
-                                               (NQT == 2 ? span_bits(m0 - 32 * k, m1 - 32 * k) : 0u);
-                            const uint32_t all = __reduce_or_sync(0xffffffffu, w);
-                            if (lane == 0) buf[4 * quad + k] = all;
-                        }
-                        __syncwarp();
-                        named_sync(1, 128);  // two buffers: the next block's words never meet late readers
-                        const uint32_t any = buf[quad] | buf[4 + quad] | buf[8 + quad] | buf[12 + quad];
-                        keep = (any >> lane) & 1u;
+                    for (int u = 0; u < 8; ++u) {
+                        z[u] = __fmul2_rn(make_float2(u2f(raw[2 * u]), u2f(raw[2 * u + 1])), in2);
+                        const float2 w = __fmul2_rn(z[u], z[u]);
+                        far = fmax3(far, w.x, w.y);
+                        z[u] = __fmul2_rn(z[u], tanh_poly(w, p.tanh_k));
                     }
-                    if (!__all_sync(0xffffffffu, keep)) {
-                        const uint32_t iV = gtile + 2 * j + 1;
-                        const int sV = (int)(iV % NS);
-                        ok = mbar_wait(kv_full(sV), (iV / NS) & 1, abort_flag, p.status, kDevErrTimeoutKV, p.gen);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        if (!keep) {
+                    // (a NaN compares false and stays a NaN in the polynomial)
+                    if (__any_sync(0xffffffffu, far > kTanhMaxSq)) {
 #pragma unroll
-                            for (int b = 0; b < NBOX_D; ++b)
-#pragma unroll
-                                for (int v = 0; v < 8; ++v)
-                                    st_shared_v4(sKV + sV * C::KVTILE + b * (kBN * 128) + r * 128 + v * 16, 0.f, 0.f, 0.f,
-                                                 0.f);
+                        for (int u = 0; u < 8; ++u) {
+                            z[u].x = cap_far(u2f(raw[2 * u]) * p.cap_in, z[u].x, p.cap_out);
+                            z[u].y = cap_far(u2f(raw[2 * u + 1]) * p.cap_in, z[u].y, p.cap_out);
                         }
-                        fence_proxy_async_smem();
+                    }
+                    if (!kBias)
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) z[u] = __fadd2_rn(z[u], add2);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        z[u] = __ffma2_rn(make_float2(u2f(raw[2 * u]), u2f(raw[2 * u + 1])), c2,
+                                          kBias ? make_float2(0.f, 0.f) : add2);
+                }
+                if constexpr (kBias) {
+                    if (past || ahead) {
+                        const float2 at = __ffma2_rn(make_float2((float)c0, (float)c0), bs2, b02);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            z[u] = __fadd2_rn(z[u], __ffma2_rn(make_float2(2.f * u, 2.f * u + 1.f), bs2, at));
+                    } else {
+                        const float d0 = (float)(key0 + c0 - qpos), fnear = (float)near;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            z[u].x += fmaf(-slope2, fabsf(d0 + 2.f * u) - fnear, add);
+                            z[u].y += fmaf(-slope2, fabsf(d0 + 2.f * u + 1.f) - fnear, add);
+                        }
                     }
                 }
+                if (!full) {
+                    const int a0 = n0 - c0, a1 = n1 - c0;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (2 * u < a0 || 2 * u >= a1) z[u].x = -INFINITY;
+                        if (2 * u + 1 < a0 || 2 * u + 1 >= a1) z[u].y = -INFINITY;
+                    }
+                }
+            };
+            // Visits the tile's chunks in order: visit(c0, raw scores); the next chunk's load runs under it.
+            auto chunks = [&](auto visit) {
+                uint32_t ra[16], rb[16];
+                tmem_ld16p(tS, ra);
+#pragma unroll 1
+                for (int c0 = 0; c0 < kBN; c0 += 32) {
+                    tmem_ld16_nowait(tS + c0 + 16, rb);
+                    visit(c0, ra);
+                    tmem_wait_ld16(rb);
+                    if (c0 + 32 < kBN) tmem_ld16_nowait(tS + c0 + 32, ra);
+                    visit(c0 + 16, rb);
+                    if (c0 + 32 < kBN) tmem_wait_ld16(ra);
+                }
+            };
+            float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+            // P of one chunk from z - m: row sums, bf16, into the first half of the score columns
+            auto weigh = [&](int c0, const float2 *x) {
+                uint32_t pk[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    float2 pr;
+                    pr.x = ex2(x[u].x);
+                    pr.y = ex2(x[u].y);
+                    if (u & 1)
+                        acc1 = __fadd2_rn(acc1, pr);
+                    else
+                        acc0 = __fadd2_rn(acc0, pr);
+                    pk[u] = pack_bf16x2(pr.x, pr.y);
+                }
+                tmem_st8(tS + (c0 >> 1), pk);
+            };
+            bool general = !none && !fixed;
+            if (none) {
+                uint32_t zero[16];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) zero[u] = 0u;
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc) tmem_st16(tS + cc * 16, zero);
+            } else if (fixed) {
+                chunks([&](int c0, const uint32_t *raw) {
+                    float2 x[8];
+                    scores(raw, c0, -p.cap_ref, x);
+                    weigh(c0, x);
+                });
+                l += (acc0.x + acc1.x) + (acc0.y + acc1.y);
+            } else if (spec) {
+                if constexpr (!kCap) {
+                    uint32_t sr[128];
+                    const float t0 = b0 - m;
+                    const float2 bs2 = make_float2(bs, bs), t02 = make_float2(t0, t0);
+                    tmem_ld16p(tS, sr);
+#pragma unroll
+                    for (int cc = 0; cc < 8; ++cc) {
+                        float2 x[8];
+                        if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int c = 16 * cc + 2 * u;
+                            const float2 at = kBias ? __ffma2_rn(make_float2((float)c, (float)(c + 1)), bs2, t02) : t02;
+                            x[u] = __ffma2_rn(make_float2(u2f(sr[c]), u2f(sr[c + 1])), c2, at);
+                        }
+                        weigh(16 * cc, x);
+                        if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
+                    }
+                    const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
+                    general = __any_sync(0xffffffffu, rs > kRedoSum);
+                    if (!general) {
+                        l += rs;
+                    } else {  // the raw scores go back under the P stored over them
+                        tmem_wait_st();
+#pragma unroll
+                        for (int cc = 0; cc < 4; ++cc)
+                            tmem_st32(tS + 32 * cc, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * cc));
+                        tmem_wait_st();
+                        acc0 = acc1 = make_float2(0.f, 0.f);
+                    }
+                }
+            }
+            if (general) {
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+                chunks([&](int c0, const uint32_t *raw) {
+                    float2 z[8];
+                    scores(raw, c0, 0.f, z);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (u & 1)
+                            mx1 = fmax3(mx1, z[u].x, z[u].y);
+                        else
+                            mx0 = fmax3(mx0, z[u].x, z[u].y);
+                    }
+                });
+                const float mb = fmaxf(mx0, mx1);
+                float m_new = m;
+                if (mb > m && (m == -INFINITY || mb - m > kRescaleLog2)) m_new = mb;
+                const float alpha = (m_new == m) ? 1.f : ((m == -INFINITY) ? 0.f : ex2(m - m_new));
+                const float ref = (m_new == -INFINITY) ? 0.f : m_new;
+                chunks([&](int c0, const uint32_t *raw) {
+                    float2 z[8];
+                    scores(raw, c0, 0.f, z);  // then the subtraction: a row's largest weighs exactly 1
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) z[u] = __fadd2_rn(z[u], make_float2(-ref, -ref));
+                    weigh(c0, z);
+                });
+                l = l * alpha + ((acc0.x + acc1.x) + (acc0.y + acc1.y));
+                m = m_new;
+                // O_t holds P V through the block before (complete: these scores were committed after it).
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                    for (int cc = 0; cc < DP / 32; ++cc) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + cc * 32, o);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[u] = f2u(u2f(o[u]) * alpha);
+                        tmem_st32(tO + cc * 32, o);
+                    }
+                }
+            }
+            // V rows that no row of the unit sees (what an unused slot holds, a key between two
+            // ranges) become zero before P V reads them: 0 * NaN would reach every row. PV_0 is
+            // issued first, after every thread of this warpgroup arrived.
+            if (t == 0 && (key0 < it.ilo || key0 + kBN > it.ihi)) {
+                bool keep = key0 + r >= it.ulo && key0 + r < it.uhi;
+                if (p.key_begin || p.key_end) {
+                    // the union of both tiles' rows as 128 bits, a word per 32 keys
+                    uint32_t *buf = seen_bits + 16 * (seen_turn & 1);
+                    ++seen_turn;
+                    const int m0 = max(lo_b - key0, 0), m1 = min(hi_b - key0, kBN);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t w = span_bits(n0 - 32 * k, n1 - 32 * k) |
+                                           (NQT == 2 ? span_bits(m0 - 32 * k, m1 - 32 * k) : 0u);
+                        const uint32_t all = __reduce_or_sync(0xffffffffu, w);
+                        if (lane == 0) buf[4 * quad + k] = all;
+                    }
+                    __syncwarp();
+                    named_sync(1, 128);  // two buffers: the next block's words never meet late readers
+                    const uint32_t any = buf[quad] | buf[4 + quad] | buf[8 + quad] | buf[12 + quad];
+                    keep = (any >> lane) & 1u;
+                }
+                if (!__all_sync(0xffffffffu, keep)) {
+                    const uint32_t iV = gtile + 2 * j + 1;
+                    const int sV = (int)(iV % NS);
+                    ok = mbar_wait(kv_full(sV), (iV / NS) & 1, abort_flag, p.status, kDevErrTimeoutKV, p.gen);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (!keep) {
+#pragma unroll
+                        for (int b = 0; b < NBOX_D; ++b)
+#pragma unroll
+                            for (int v = 0; v < 8; ++v)
+                                st_shared_v4(sKV + sV * C::KVTILE + b * (kBN * 128) + r * 128 + v * 16, 0.f, 0.f, 0.f,
+                                             0.f);
+                    }
+                    fence_proxy_async_smem();
+                }
+            }
             }
             tmem_wait_st();
             tc_fence_before();
@@ -1116,6 +1247,41 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                         bulk_commit();
                     }
                 }
+            } else if (MOD != 0 && NQT == 2 && to_o && out_bf16 && p.o_tma) {
+                // The same with bf16: a box is [32 rows][64 bf16].
+                const uint32_t buf = sO + (uint32_t)(warp - 4) * C::OSTAGE;
+                const int y0 = row0 + t * kBM + quad * 32;
+#pragma unroll
+                for (int cc = 0; cc < DP / 64; ++cc) {
+                    if (cc * 64 >= D) break;
+                    uint32_t w[32];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t o[32];
+                        if (have_o) {
+                            tmem_ld32(tO + cc * 64 + h * 32, o);
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) o[u] = 0u;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 16; ++u)
+                            w[16 * h + u] = f32_to_bf16_bits(u2f(o[2 * u]) * mult) |
+                                            (f32_to_bf16_bits(u2f(o[2 * u + 1]) * mult) << 16);
+                    }
+                    if (lane == 0) bulk_wait_read0();  // the previous box has been read out
+                    __syncwarp();
+#pragma unroll
+                    for (int v = 0; v < 8; ++v)
+                        st_shared_v4(buf + lane * 128 + ((v ^ (lane & 7)) << 4), u2f(w[4 * v]), u2f(w[4 * v + 1]),
+                                     u2f(w[4 * v + 2]), u2f(w[4 * v + 3]));
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && y0 < p.rows_per_kv) {
+                        tma_store_3d(&tmO, buf, cc * 64, y0, kv);
+                        bulk_commit();
+                    }
+                }
             } else if (out_bf16) {
                 store_rows(std::true_type{});
             } else {
@@ -1149,17 +1315,19 @@ static EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// The fp32 output as a 3-D tensor map {D, rows_per_kv, Hkv} (the layout of Q) for the epilogue's
-// TMA stores: boxes of [32 rows][32 floats], 128-byte swizzle.
-static bool make_map_o(CUtensorMap *m, float *O, uint64_t D, uint64_t rows, uint64_t hkv) {
+// The output as a 3-D tensor map {D, rows_per_kv, Hkv} (the layout of Q) for the epilogue's TMA
+// stores: boxes of 32 rows and 128 bytes (32 fp32 or 64 bf16), 128-byte swizzle.
+static bool make_map_o(CUtensorMap *m, float *O, bool bf16, uint64_t D, uint64_t rows, uint64_t hkv) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
+    const uint64_t size = bf16 ? 2 : 4;
     cuuint64_t dims[3] = {D, rows, hkv};
-    cuuint64_t strides[2] = {D * 4, rows * D * 4};
-    cuuint32_t box[3] = {32, 32, 1};
+    cuuint64_t strides[2] = {D * size, rows * D * size};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, O, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, O, dims, strides, box,
+                    estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
 
@@ -1234,10 +1402,10 @@ static int launch_tc(const fa_problem *P, cudaStream_t st, int tiles_per_kv) {
     }
     CUtensorMap tmO;
     memset(&tmO, 0, sizeof tmO);
-    // fp32 normalised output of a two-tile instance: stored by TMA (any other output keeps per-row
-    // stores)
-    const int o_tma = NQT == 2 && P->O != nullptr && !P->o_bf16 && !P->write_partials;
-    if (o_tma && !make_map_o(&tmO, P->O, D, rows, (uint64_t)P->Hkv)) return ATTN_ERR_CUDA;
+    // normalised output of a two-tile instance: stored by TMA (bf16 with modified scores only; any other
+    // output keeps per-row stores)
+    const int o_tma = NQT == 2 && P->O != nullptr && (MOD != 0 || !P->o_bf16) && !P->write_partials;
+    if (o_tma && !make_map_o(&tmO, P->O, P->o_bf16 != 0, D, rows, (uint64_t)P->Hkv)) return ATTN_ERR_CUDA;
     TcParams prm;
     prm.O = P->O;
     prm.o_tma = o_tma;
@@ -1281,6 +1449,8 @@ static int launch_tc(const fa_problem *P, cudaStream_t st, int tiles_per_kv) {
     prm.slopes = P->slopes;
     prm.cap_in = P->cap_in;
     prm.cap_out = P->cap_out;
+    prm.cap_ref = P->cap_out > 0.f && P->cap_out <= 75.f ? (P->cap_out > 50.f ? P->cap_out - 50.f : 0.f) : -1.f;
+    for (int i = 0; i < 6; ++i) prm.tanh_k[i] = P->cap_out * kTanhC[i];
     prm.group = group;
     prm.head_units = (P->Sq % (kBM * NQT) == 0) ? P->Sq / (kBM * NQT) : 0;
     const int sms = ts_num_sms() > 0 ? ts_num_sms() : 1;

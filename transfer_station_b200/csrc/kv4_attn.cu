@@ -60,7 +60,7 @@ struct Kv4Params {
     int B, Hq, Hkv, Sq, group, row_blocks, causal;
     int page_size, num_pages, max_pages;
     float scale_log2;  // log2(e) / sqrt(D)
-    float cap_in, cap_out;
+    float cap_in, cap_out, tanh_k[6];
     const float *slopes;
     const int *key_begin, *key_end;
     int *status;                  // [0]: result; [2], [3]: reports of the running call and its generation
@@ -487,7 +487,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 for (int e = 0; e < 4; ++e) {
                     const int c = e & 1;
                     float z = s[n][e] * fac[n][c];
-                    if (has_cap) z = cap_exact(z, p.cap_out);
+                    if (has_cap) {
+                        const float w = z * z;
+                        z = cap_far(z, z * tanh_poly(make_float2(w, w), p.tanh_k).x, p.cap_out);
+                    }
                     const int key = key0 + g + 8 * (e >> 1);
                     if (has_bias) z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
                     if (!whole && (key < lo[n][c] || key >= hi[n][c])) z = -INFINITY;
@@ -770,6 +773,7 @@ int run(const ts_kv4_problem *P, cudaStream_t st) {
     p.page_size = P->page_size, p.num_pages = P->num_pages, p.max_pages = P->max_pages;
     p.scale_log2 = P->scale_log2;
     p.cap_in = P->cap_in, p.cap_out = P->cap_out;
+    for (int i = 0; i < 6; ++i) p.tanh_k[i] = P->cap_out * kTanhC[i];
     p.slopes = P->slopes;
     p.key_begin = P->key_begin, p.key_end = P->key_end;
     p.status = P->status;
