@@ -101,7 +101,11 @@ struct TcParams {
     float cap_in;         // 1 / (cap * sqrt(D)): raw score -> argument of tanh
     float cap_out;        // cap * log2(e)
     float cap_ref;        // the fixed reference of capped scores, or negative: a running maximum
-    float tanh_k[6];      // cap_out times the tanh polynomial's coefficients
+    // The tanh polynomial's coefficients times cap_out; with a fixed reference also times cap_in^(2i+1),
+    // so that the polynomial takes the raw score itself (cap_in is then within [1e-3, 400]: no power
+    // of it leaves fp32's range).
+    float tanh_k[5];
+    float far_sq;         // the square of the raw score (or of y) past which the polynomial ends
 };
 
 // What MOD adds to the scores (every MOD != 0 also has the key ranges).
@@ -935,30 +939,30 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             if (!ok) break;
             tc_fence_after();
             // 16 columns from c0: raw scores -> z + add (-inf outside the row's keys)
-            auto scores = [&](const uint32_t *raw, int c0, float add, float2 *z) {
+            auto scores = [&](auto raw_tag, const uint32_t *raw, int c0, float add, float2 *z) {
                 const float2 add2 = make_float2(add, add), bs2 = make_float2(bs, bs);
                 const float2 b02 = make_float2(b0 + add, b0 + add);
                 if constexpr (kCap) {
+                    constexpr bool kRaw = decltype(raw_tag)::value;  // the polynomial takes raw scores
                     const float2 in2 = make_float2(p.cap_in, p.cap_in);
+                    const float2 end2 = kBias ? make_float2(0.f, 0.f) : add2;
                     float far = 0.f;
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
-                        z[u] = __fmul2_rn(make_float2(u2f(raw[2 * u]), u2f(raw[2 * u + 1])), in2);
-                        const float2 w = __fmul2_rn(z[u], z[u]);
+                        const float2 r = make_float2(u2f(raw[2 * u]), u2f(raw[2 * u + 1]));
+                        const float2 y = kRaw ? r : __fmul2_rn(r, in2);
+                        const float2 w = __fmul2_rn(y, y);
                         far = fmax3(far, w.x, w.y);
-                        z[u] = __fmul2_rn(z[u], tanh_poly(w, p.tanh_k));
+                        z[u] = __ffma2_rn(y, tanh_poly(w, p.tanh_k), end2);
                     }
                     // (a NaN compares false and stays a NaN in the polynomial)
-                    if (__any_sync(0xffffffffu, far > kTanhMaxSq)) {
+                    if (__any_sync(0xffffffffu, far > p.far_sq)) {
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
-                            z[u].x = cap_far(u2f(raw[2 * u]) * p.cap_in, z[u].x, p.cap_out);
-                            z[u].y = cap_far(u2f(raw[2 * u + 1]) * p.cap_in, z[u].y, p.cap_out);
+                            z[u].x = cap_far(u2f(raw[2 * u]) * p.cap_in, z[u].x, p.cap_out, end2.x);
+                            z[u].y = cap_far(u2f(raw[2 * u + 1]) * p.cap_in, z[u].y, p.cap_out, end2.x);
                         }
                     }
-                    if (!kBias)
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) z[u] = __fadd2_rn(z[u], add2);
                 } else {
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
@@ -1030,7 +1034,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             } else if (fixed) {
                 chunks([&](int c0, const uint32_t *raw) {
                     float2 x[8];
-                    scores(raw, c0, -p.cap_ref, x);
+                    scores(std::true_type{}, raw, c0, -p.cap_ref, x);
                     weigh(c0, x);
                 });
                 l += (acc0.x + acc1.x) + (acc0.y + acc1.y);
@@ -1071,7 +1075,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 float mx0 = -INFINITY, mx1 = -INFINITY;
                 chunks([&](int c0, const uint32_t *raw) {
                     float2 z[8];
-                    scores(raw, c0, 0.f, z);
+                    scores(std::false_type{}, raw, c0, 0.f, z);
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
                         if (u & 1)
@@ -1087,7 +1091,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 const float ref = (m_new == -INFINITY) ? 0.f : m_new;
                 chunks([&](int c0, const uint32_t *raw) {
                     float2 z[8];
-                    scores(raw, c0, 0.f, z);  // then the subtraction: a row's largest weighs exactly 1
+                    scores(std::false_type{}, raw, c0, 0.f, z);  // then the subtraction: a row's largest weighs exactly 1
 #pragma unroll
                     for (int u = 0; u < 8; ++u) z[u] = __fadd2_rn(z[u], make_float2(-ref, -ref));
                     weigh(c0, z);
@@ -1450,7 +1454,10 @@ static int launch_tc(const fa_problem *P, cudaStream_t st, int tiles_per_kv) {
     prm.cap_in = P->cap_in;
     prm.cap_out = P->cap_out;
     prm.cap_ref = P->cap_out > 0.f && P->cap_out <= 75.f ? (P->cap_out > 50.f ? P->cap_out - 50.f : 0.f) : -1.f;
-    for (int i = 0; i < 6; ++i) prm.tanh_k[i] = P->cap_out * kTanhC[i];
+    float power = prm.cap_ref >= 0.f ? P->cap_in : 1.f;
+    prm.far_sq = kTanhMaxSq / (power * power);
+    for (int i = 0; i < 5; ++i, power *= prm.cap_ref >= 0.f ? P->cap_in * P->cap_in : 1.f)
+        prm.tanh_k[i] = P->cap_out * kTanhC[i] * power;
     prm.group = group;
     prm.head_units = (P->Sq % (kBM * NQT) == 0) ? P->Sq / (kBM * NQT) : 0;
     const int sms = ts_num_sms() > 0 ? ts_num_sms() : 1;

@@ -60,7 +60,7 @@ struct Kv4Params {
     int B, Hq, Hkv, Sq, group, row_blocks, causal;
     int page_size, num_pages, max_pages;
     float scale_log2;  // log2(e) / sqrt(D)
-    float cap_in, cap_out, tanh_k[6];
+    float cap_in, cap_out, tanh_k[5];
     const float *slopes;
     const int *key_begin, *key_end;
     int *status;                  // [0]: result; [2], [3]: reports of the running call and its generation
@@ -773,7 +773,7 @@ int run(const ts_kv4_problem *P, cudaStream_t st) {
     p.page_size = P->page_size, p.num_pages = P->num_pages, p.max_pages = P->max_pages;
     p.scale_log2 = P->scale_log2;
     p.cap_in = P->cap_in, p.cap_out = P->cap_out;
-    for (int i = 0; i < 6; ++i) p.tanh_k[i] = P->cap_out * kTanhC[i];
+    for (int i = 0; i < 5; ++i) p.tanh_k[i] = P->cap_out * kTanhC[i];
     p.slopes = P->slopes;
     p.key_begin = P->key_begin, p.key_end = P->key_end;
     p.status = P->status;
