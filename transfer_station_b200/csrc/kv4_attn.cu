@@ -24,7 +24,7 @@
 // takes the c-th G-th of it, whatever the lengths are, so a ragged batch stays balanced without the host
 // knowing a length. A unit cut between CTAs leaves (m, l, acc) partials, merged by kv4_combine.
 // One producer warp per CTA streams tiles into a ring of shared-memory stages with untiled bulk copies;
-// four consumer warps take 16 keys of each tile, each with its own running maximum and accumulator, merged
+// four consumer warps take 32 keys of each tile, each with its own running maximum and accumulator, merged
 // in shared memory at a unit's end.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -44,10 +44,11 @@ namespace ts {
 
 namespace {
 
-constexpr int kTile = 64;        // keys per stage
-constexpr int kWarps = 4;        // consumer warps, 16 keys of a tile each
+constexpr int kTile = 128;       // keys per stage
+constexpr int kWarps = 4;        // consumer warps, 32 keys of a tile each
+constexpr int kSlabs = 2;        // 16-key MMA rows of a warp and tile
 constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kMinTiles = 2;     // a CTA takes at least this many tiles (fewer CTAs work on small problems)
+constexpr int kMinTiles = 1;     // a CTA takes at least this many tiles (fewer CTAs work on small problems)
 
 constexpr float kHead = 7.f, kMost = 15.f;  // see the weights
 
@@ -73,7 +74,7 @@ template <int D, int NT>
 struct Kv4Config {
     static constexpr int CODES = kTile * D / 2, SCALES = kTile * D / ATTN_KV4_GROUP;
     static constexpr int STAGE = 2 * (CODES + SCALES);
-    static constexpr int NS = D == 128 ? 5 : 8;
+    static constexpr int NS = D == 128 ? 3 : 6;
     static constexpr int ROWS = 8 * NT;
     static constexpr int MERGE = kWarps * ROWS * (D + 4) * 4;  // one warp's accumulator rows, padded
     static constexpr int OFF_MERGE = NS * STAGE;
@@ -112,12 +113,18 @@ struct Dequant {
           lo_add(__hmul2(s, __float2half2_rn(-64.5f))),
           hi(__hmul2(s, __float2half2_rn(1.f / 256.f))),
           hi_add(__hmul2(s, __float2half2_rn(-4.5f))) {}
+    // (x & mask) | 1024's exponent in one LOP3: written out, the compiler emits two with an immediate each
+    __device__ __forceinline__ static uint32_t place(uint32_t x, uint32_t mask) {
+        uint32_t r;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(0x64006400u));
+        return r;
+    }
     // nibbles at bits 0 and 16, and at bits 4 and 20
     __device__ __forceinline__ uint32_t low(uint32_t x) const {
-        return as_u32(__hfma2(as_half2((x & 0x000f000fu) | 0x64006400u), lo, lo_add));
+        return as_u32(__hfma2(as_half2(place(x, 0x000f000fu)), lo, lo_add));
     }
     __device__ __forceinline__ uint32_t high(uint32_t x) const {
-        return as_u32(__hfma2(as_half2((x & 0x00f000f0u) | 0x64006400u), hi, hi_add));
+        return as_u32(__hfma2(as_half2(place(x, 0x00f000f0u)), hi, hi_add));
     }
 };
 
@@ -248,7 +255,8 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
-template <int D, int NT>
+// MOD: the call has a cap, a bias or key ranges.
+template <int D, int NT, bool MOD>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv4Params p) {
     using C = Kv4Config<D, NT>;
     constexpr int KW = D / 32;             // 32-bit words of a key row that a lane holds (its quarter of the row)
@@ -284,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
         const int P = p.page_size;
         const int rows = P < kTile ? P : kTile;      // keys per copy
         const int per_tile = kTile / rows;           // copies per pool and tile
-        long long k = 0;                             // tiles issued
+        int st = 0;                                  // next stage, and the round of the ring it is in
+        uint32_t round = 0;
         bool ok = true;
         while (left > 0 && ok) {
             const Span sp = seq_span(p, b);
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
             const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
             // chunk ids (a chunk: `rows` keys) of the next 32 chunks, one a lane
             int win = -1, id = -1;
-            for (int i = tile; i < end && ok; ++i, ++k) {
+            for (int i = tile; i < end && ok; ++i) {
                 const int c0 = (sp.t0 + i) * per_tile;
                 if (win < 0 || c0 + per_tile > win + 32) {
                     win = c0;
@@ -310,8 +319,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                         }
                     }
                 }
-                const int st = (int)(k % C::NS);
-                const uint32_t round = (uint32_t)(k / C::NS);
                 if (round > 0) ok = ring_wait(empty(st), (round - 1) & 1u, abort_flag, p, kDevErrTimeoutKV);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -331,6 +338,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                     bulk_load(dst + 2 * C::CODES + C::SCALES + lane * scale_bytes, p.vs + at * GROUPS, scale_bytes, bar);
                 }
                 __syncwarp();
+                if (++st == C::NS) {
+                    st = 0;
+                    ++round;
+                }
             }
             left -= end - tile;
             tile = 0;
@@ -340,9 +351,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
             }
         }
         // copies in flight land before the CTA exits: the last issue of each stage
-        for (long long j = k > C::NS ? k - C::NS : 0; j < k; ++j) {
+        for (int j = 0; j < C::NS; ++j) {
             volatile int never = 0;
-            ring_wait(full((int)(j % C::NS)), (uint32_t)(j / C::NS) & 1u, &never, p, kDevErrTimeoutDrain);
+            if (j < st)
+                ring_wait(full(j), round & 1u, &never, p, kDevErrTimeoutDrain);
+            else if (round > 0)
+                ring_wait(full(j), (round - 1) & 1u, &never, p, kDevErrTimeoutDrain);
         }
         return;
     }
@@ -352,8 +366,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
     float *merge = reinterpret_cast<float *>(smem + C::OFF_MERGE);
     float *ml = reinterpret_cast<float *>(smem + C::OFF_ML);
     const int rows_all = p.group * p.Sq;
-    const bool has_cap = p.cap_out > 0.f, has_bias = p.slopes != nullptr;
-    long long k = 0;
+    const bool has_cap = MOD && p.cap_out > 0.f, has_bias = MOD && p.slopes != nullptr;
+    int st = 0;
+    uint32_t phase = 0;
     bool ok = true;
     while (left > 0) {
         const Span span = seq_span(p, b);
@@ -428,10 +443,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
 
-        float m[NT][2], l[NT][2], acc[NT][MT][4];
+        float ref[NT][2], most[NT][2], l[NT][2], acc[NT][MT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
+            ref[n][0] = ref[n][1] = 0.f;
+            most[n][0] = most[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -439,140 +455,170 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 for (int c = 0; c < 4; ++c) acc[n][i][c] = 0.f;
         }
 
-        for (int i = begin; i < end; ++i, ++k) {
-            const int st = (int)(k % C::NS);
-            if (ok) ok = ring_wait(full(st), (uint32_t)(k / C::NS) & 1u, abort_flag, p, kDevErrTimeoutKV);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+        for (int i = begin; i < end; ++i) {
+            if (!__all_sync(0xffffffffu, ok && mbar_try_wait(full(st), phase))) {
+                if (ok) ok = ring_wait(full(st), phase, abort_flag, p, kDevErrTimeoutKV);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
             const uint8_t *stage = smem + st * C::STAGE;
-            const int key0 = (span.t0 + i) * kTile + 16 * warp;            // this warp's 16 keys
-            const bool edge = key0 < span.lo || key0 + 16 > span.hi;       // some are not the sequence's to see
-            // ---- S^T = K Q^T
-            float s[NT][4];
+            const int key0 = (span.t0 + i) * kTile + 16 * kSlabs * warp;  // this warp's keys
+            if (key0 < span.hi && key0 + 16 * kSlabs > span.lo) {
+                // ---- S^T = K Q^T
+                float s[kSlabs][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            {
-                const int r0 = 16 * warp + g;
-                const uint8_t *rowp = stage + r0 * (D / 2) + t * (D / 8);
-                uint32_t ka[KW], kb[KW];
-                if constexpr (KW == 4) {
-                    *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(rowp);
-                    *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(rowp + 8 * (D / 2));
-                } else {
-                    *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(rowp);
-                    *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(rowp + 8 * (D / 2));
-                }
-                const uint8_t *sp = stage + C::CODES + r0 * GROUPS + t * GROUPS / 4;
-                const uint32_t sa = sp[0], sb = sp[8 * GROUPS];
-                const Dequant da(scales2(sa, sa)), db(scales2(sb, sb));
+                for (int b = 0; b < kSlabs; ++b) {
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    uint32_t x = ka[w], y = kb[w];
-                    uint32_t a[4] = {da.low(x), db.low(y), da.high(x), db.high(y)};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816(s[n], a, qf[n][2 * w][0], qf[n][2 * w][1]);
-                    x >>= 8;
-                    y >>= 8;
-                    a[0] = da.low(x), a[1] = db.low(y), a[2] = da.high(x), a[3] = db.high(y);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816(s[n], a, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
-                }
-            }
-            // ---- scores in log2 units: element e of s is key g + 8 (e / 2), query column e % 2
-            const bool whole = key0 >= all_lo && key0 + 16 <= all_hi;
-            bool above = false;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = e & 1;
-                    float z = s[n][e] * fac[n][c];
-                    if (has_cap) {
-                        const float w = z * z;
-                        z = cap_far(z, z * tanh_poly(make_float2(w, w), p.tanh_k).x, p.cap_out);
+                    for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+                    const int r0 = 16 * (kSlabs * warp + b) + g;
+                    const uint8_t *rowp = stage + r0 * (D / 2) + t * (D / 8);
+                    uint32_t ka[KW], kb[KW];
+                    if constexpr (KW == 4) {
+                        *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(rowp);
+                        *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(rowp + 8 * (D / 2));
+                    } else {
+                        *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(rowp);
+                        *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(rowp + 8 * (D / 2));
                     }
-                    const int key = key0 + g + 8 * (e >> 1);
-                    if (has_bias) z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
-                    if (!whole && (key < lo[n][c] || key >= hi[n][c])) z = -INFINITY;
-                    s[n][e] = z;
-                    above |= z > m[n][c] + kMost;
-                }
-            // A column's reference m is its maximum less kHead when it was set, and moves only when a score
-            // exceeds m + kMost. Weights 2^(z - m) thus reach from 2^kHead at the maximum up to 2^kMost,
-            // inside fp16's range, and keep 11 bits down to 2^-(14 + kHead) of the largest; below that the
-            // step is 2^-(24 + kHead) of it.
-            if (__any_sync(0xffffffffu, above)) {
+                    const uint8_t *sp = stage + C::CODES + r0 * GROUPS + t * GROUPS / 4;
+                    const uint32_t sa = sp[0], sb = sp[8 * GROUPS];
+                    const Dequant da(scales2(sa, sa)), db(scales2(sb, sb));
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int w = 0; w < KW; ++w) {
+                        uint32_t x = ka[w], y = kb[w];
+                        uint32_t a[4] = {da.low(x), db.low(y), da.high(x), db.high(y)};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float mx = fmaxf(s[n][c], s[n][c + 2]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float to = fmaxf(m[n][c], mx - kHead);
-                        const float alpha = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - to);
-                        m[n][c] = to;
-                        l[n][c] *= alpha;
-#pragma unroll
-                        for (int q = 0; q < MT; ++q) {
-                            acc[n][q][c] *= alpha;
-                            acc[n][q][c + 2] *= alpha;
-                        }
-                    }
-            }
-            // ---- weights, and their transpose as the B operand of O^T += V^T P^T
-            uint32_t pf[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mm = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1];
-                    w[e] = ex2(s[n][e] - mm);
-                    l[n][e & 1] += w[e];
-                }
-                pf[n][0] = transpose8x8(as_u32(__floats2half2_rn(w[0], w[1])));
-                pf[n][1] = transpose8x8(as_u32(__floats2half2_rn(w[2], w[3])));
-            }
-            // ---- V^T: rows are this lane's D/8 elements, columns keys 2t, 2t+1, 2t+8, 2t+9
-            {
-                const uint8_t *vp = stage + C::CODES + C::SCALES + (16 * warp + 2 * t) * (D / 2) + g * (D / 16);
-                const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + (16 * warp + 2 * t) * GROUPS + g * GROUPS / 8;
-                uint32_t v[4][VW];
-                uint32_t sc[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = (j & 1) + 8 * (j >> 1);
-                    if constexpr (VW == 2)
-                        *reinterpret_cast<uint2 *>(v[j]) = *reinterpret_cast<const uint2 *>(vp + r * (D / 2));
-                    else
-                        v[j][0] = *reinterpret_cast<const uint32_t *>(vp + r * (D / 2));
-                    sc[j] = sp[r * GROUPS];
-                    // what an unseen slot holds may be any byte, a NaN scale among them: it becomes zero
-                    if (edge && (key0 + 2 * t + r < span.lo || key0 + 2 * t + r >= span.hi)) sc[j] = 0u;
-                }
-                const Dequant d0(scales2(sc[0], sc[1])), d1(scales2(sc[2], sc[3]));
-#pragma unroll
-                for (int w = 0; w < VW; ++w)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // the same half word of both keys: nibble n of each half is element 8w + 4h + n
-                        uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
-                        uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
-                        uint32_t a[4] = {d0.low(x), d0.high(x), d1.low(y), d1.high(y)};
-                        const int i0 = 4 * w + 2 * h;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816(acc[n][i0], a, pf[n][0], pf[n][1]);
+                        for (int n = 0; n < NT; ++n) mma16816(s[b][n], a, qf[n][2 * w][0], qf[n][2 * w][1]);
                         x >>= 8;
                         y >>= 8;
-                        a[0] = d0.low(x), a[1] = d0.high(x), a[2] = d1.low(y), a[3] = d1.high(y);
+                        a[0] = da.low(x), a[1] = db.low(y), a[2] = da.high(x), a[3] = db.high(y);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816(acc[n][i0 + 1], a, pf[n][0], pf[n][1]);
+                        for (int n = 0; n < NT; ++n) mma16816(s[b][n], a, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
                     }
+                }
+                // ---- scores less their column's reference, log2 units: element e is key g + 8 (e / 2) of its
+                // slab, query column e % 2
+                const bool whole = key0 >= all_lo && key0 + 16 * kSlabs <= all_hi;
+                bool above = false;
+#pragma unroll
+                for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int c = e & 1;
+                            float z;
+                            if (has_cap) {
+                                const float y = s[b][n][e] * fac[n][c], w = y * y;
+                                z = cap_far(y, y * tanh_poly(make_float2(w, w), p.tanh_k).x, p.cap_out) - ref[n][c];
+                            } else {
+                                z = fmaf(s[b][n][e], fac[n][c], -ref[n][c]);
+                            }
+                            const int key = key0 + 16 * b + g + 8 * (e >> 1);
+                            if (has_bias)
+                                z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
+                            if (!whole && (key < lo[n][c] || key >= hi[n][c])) z = -INFINITY;
+                            s[b][n][e] = z;
+                            above |= z > most[n][c];
+                        }
+                // A column's reference is its maximum less kHead when it was set, and moves only when a score
+                // exceeds it by kMost. Weights 2^z thus reach from 2^kHead at the maximum up to 2^kMost, inside
+                // fp16's range, and keep 11 bits down to 2^-(14 + kHead) of the largest; below that the step is
+                // 2^-(24 + kHead) of it. (Until a column has seen a key, most is -inf and the reference 0.)
+                if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float mx = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+                            for (int b = 1; b < kSlabs; ++b) mx = fmax3(mx, s[b][n][c], s[b][n][c + 2]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            const bool first = most[n][c] == -INFINITY;
+                            if (mx == -INFINITY) continue;  // (uniform over the column's lanes)
+                            const float by = first ? mx - kHead : fmaxf(0.f, mx - kHead);
+                            const float alpha = first ? 0.f : ex2(-by);
+                            ref[n][c] += by;
+                            most[n][c] = kMost;
+                            l[n][c] *= alpha;
+#pragma unroll
+                            for (int b = 0; b < kSlabs; ++b) {
+                                s[b][n][c] -= by;
+                                s[b][n][c + 2] -= by;
+                            }
+#pragma unroll
+                            for (int q = 0; q < MT; ++q) {
+                                acc[n][q][c] *= alpha;
+                                acc[n][q][c + 2] *= alpha;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int b = 0; b < kSlabs; ++b) {
+                    // ---- weights, and their transpose as the B operand of O^T += V^T P^T
+                    uint32_t pf[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = ex2(s[b][n][e]);
+                            l[n][e & 1] += w[e];
+                        }
+                        pf[n][0] = transpose8x8(as_u32(__floats2half2_rn(w[0], w[1])));
+                        pf[n][1] = transpose8x8(as_u32(__floats2half2_rn(w[2], w[3])));
+                    }
+                    // ---- V^T: rows are this lane's D/8 elements, columns keys 2t, 2t+1, 2t+8, 2t+9
+                    const int r1 = 16 * (kSlabs * warp + b) + 2 * t;
+                    const uint8_t *vp = stage + C::CODES + C::SCALES + r1 * (D / 2) + g * (D / 16);
+                    const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + r1 * GROUPS + g * GROUPS / 8;
+                    uint32_t v[4][VW];
+                    uint32_t sc[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = (j & 1) + 8 * (j >> 1);
+                        if constexpr (VW == 2)
+                            *reinterpret_cast<uint2 *>(v[j]) = *reinterpret_cast<const uint2 *>(vp + r * (D / 2));
+                        else
+                            v[j][0] = *reinterpret_cast<const uint32_t *>(vp + r * (D / 2));
+                        sc[j] = sp[r * GROUPS];
+                    }
+                    if (!whole) {
+                        // what an unseen slot holds may be any byte, a NaN scale among them: it becomes zero
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = key0 + 16 * b + 2 * t + (j & 1) + 8 * (j >> 1);
+                            if (key < span.lo || key >= span.hi) sc[j] = 0u;
+                        }
+                    }
+                    const Dequant d0(scales2(sc[0], sc[1])), d1(scales2(sc[2], sc[3]));
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            // the same half word of both keys: nibble n of each half is element 8w + 4h + n
+                            uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
+                            uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+                            uint32_t a[4] = {d0.low(x), d0.high(x), d1.low(y), d1.high(y)};
+                            const int i0 = 4 * w + 2 * h;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma16816(acc[n][i0], a, pf[n][0], pf[n][1]);
+                            x >>= 8;
+                            y >>= 8;
+                            a[0] = d0.low(x), a[1] = d0.high(x), a[2] = d1.low(y), a[3] = d1.high(y);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma16816(acc[n][i0 + 1], a, pf[n][0], pf[n][1]);
+                        }
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(st));
+            if (++st == C::NS) {
+                st = 0;
+                phase ^= 1u;
+            }
         }
 
         // ---- merge the four warps: rows [ROWS] x D
@@ -585,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
                 l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
                 if (g == 0) {
-                    ml[warp * C::ROWS + 8 * n + 2 * t + c] = m[n][c];
+                    ml[warp * C::ROWS + 8 * n + 2 * t + c] = most[n][c] == -INFINITY ? -INFINITY : ref[n][c];
                     ml[(kWarps + warp) * C::ROWS + 8 * n + 2 * t + c] = l[n][c];
                 }
                 float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (D + 4) + g * (D / 8);
@@ -735,7 +781,7 @@ int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, int smem, cudaStream_t
 }
 
 // CTAs of this kernel that fit on an SM (cached per device, with the shared-memory opt-in done).
-template <int D, int NT>
+template <int D, int NT, bool MOD>
 int resident() {
     static std::atomic<int> cache[64];
     int dev = 0;
@@ -745,7 +791,7 @@ int resident() {
         const int r = cache[dev].load(std::memory_order_acquire);
         if (r > 0) return r;
     }
-    auto kern = kv4_kernel<D, NT>;
+    auto kern = kv4_kernel<D, NT, MOD>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv4Config<D, NT>::SMEM) != cudaSuccess)
         return -1;
     int r = 0;
@@ -755,9 +801,9 @@ int resident() {
     return r;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool MOD>
 int run(const ts_kv4_problem *P, cudaStream_t st) {
-    const int fit = resident<D, NT>();
+    const int fit = resident<D, NT, MOD>();
     if (fit < 0) return ATTN_ERR_CUDA;
     Kv4Params p;
     p.Q = P->Q;
@@ -790,7 +836,7 @@ int run(const ts_kv4_problem *P, cudaStream_t st) {
     const size_t acc = (size_t)2 * ctas * 8 * NT * D;
     if (acc * 4 + (size_t)units * sizeof(int2) > (size_t)P->part_rows * D * 4) return ATTN_ERR_ARGS;
     p.desc = reinterpret_cast<int2 *>(P->part_acc + acc);
-    const int rc = launch(kv4_kernel<D, NT>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, p);
+    const int rc = launch(kv4_kernel<D, NT, MOD>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, p);
     if (rc != ATTN_OK) return rc;
     return launch(kv4_combine<D, NT>, dim3((unsigned)units, 8 * NT), dim3(128), 0, st, p);
 }
@@ -803,6 +849,11 @@ extern "C" int ts_launch_kv4(const ts_kv4_problem *P, void *stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const long long rows = (long long)(P->Hq / P->Hkv) * P->Sq;
     // up to 8 query rows of a kv head: one column tile; more: two, so that a cache row serves 16
-    if (P->D == 64) return rows <= 8 ? ts::run<64, 1>(P, st) : ts::run<64, 2>(P, st);
-    return rows <= 8 ? ts::run<128, 1>(P, st) : ts::run<128, 2>(P, st);
+    const bool mod = P->cap_out > 0.f || P->slopes || P->key_begin || P->key_end;
+    if (P->D == 64) {
+        if (mod) return rows <= 8 ? ts::run<64, 1, true>(P, st) : ts::run<64, 2, true>(P, st);
+        return rows <= 8 ? ts::run<64, 1, false>(P, st) : ts::run<64, 2, false>(P, st);
+    }
+    if (mod) return rows <= 8 ? ts::run<128, 1, true>(P, st) : ts::run<128, 2, true>(P, st);
+    return rows <= 8 ? ts::run<128, 1, false>(P, st) : ts::run<128, 2, false>(P, st);
 }
