@@ -99,9 +99,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
 
-// Two E4M3 bytes -> fp16.
-__device__ __forceinline__ __half2 scales2(uint32_t lo, uint32_t hi) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(lo | (hi << 8)), __NV_E4M3);
+// Two E4M3 bytes (the low half word) -> fp16.
+__device__ __forceinline__ __half2 scales2(uint32_t bytes) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)bytes, __NV_E4M3);
     return __half2(r);
 }
 
@@ -367,6 +367,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
     float *ml = reinterpret_cast<float *>(smem + C::OFF_ML);
     const int rows_all = p.group * p.Sq;
     const bool has_cap = MOD && p.cap_out > 0.f, has_bias = MOD && p.slopes != nullptr;
+    // byte selector of a value group's scales for a pair of keys
+    const uint32_t pick = GROUPS == 4 ? (uint32_t)((g >> 1) | ((4 + (g >> 1)) << 4)) | 0x4400u
+                                      : (uint32_t)((g >> 2) | ((2 + (g >> 2)) << 4)) | 0x4400u;
     int st = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -481,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                         *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(rowp + 8 * (D / 2));
                     }
                     const uint8_t *sp = stage + C::CODES + r0 * GROUPS + t * GROUPS / 4;
-                    const uint32_t sa = sp[0], sb = sp[8 * GROUPS];
-                    const Dequant da(scales2(sa, sa)), db(scales2(sb, sb));
+                    const __half2 sc = scales2(sp[0] | ((uint32_t)sp[8 * GROUPS] << 8));
+                    const Dequant da(__low2half2(sc)), db(__high2half2(sc));
 #pragma unroll
                     for (int w = 0; w < KW; ++w) {
                         uint32_t x = ka[w], y = kb[w];
@@ -499,7 +502,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 // ---- scores less their column's reference, log2 units: element e is key g + 8 (e / 2) of its
                 // slab, query column e % 2
                 const bool whole = key0 >= all_lo && key0 + 16 * kSlabs <= all_hi;
-                bool above = false;
 #pragma unroll
                 for (int b = 0; b < kSlabs; ++b)
 #pragma unroll
@@ -514,13 +516,33 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                             } else {
                                 z = fmaf(s[b][n][e], fac[n][c], -ref[n][c]);
                             }
-                            const int key = key0 + 16 * b + g + 8 * (e >> 1);
-                            if (has_bias)
+                            if (has_bias) {
+                                const int key = key0 + 16 * b + g + 8 * (e >> 1);
                                 z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
-                            if (!whole && (key < lo[n][c] || key >= hi[n][c])) z = -INFINITY;
+                            }
                             s[b][n][e] = z;
-                            above |= z > most[n][c];
                         }
+                if (!whole) {
+#pragma unroll
+                    for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = key0 + 16 * b + g + 8 * (e >> 1);
+                                if (key < lo[n][e & 1] || key >= hi[n][e & 1]) s[b][n][e] = -INFINITY;
+                            }
+                }
+                bool above = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+                        for (int b = 1; b < kSlabs; ++b) mx = fmax3(mx, s[b][n][c], s[b][n][c + 2]);
+                        above |= mx > most[n][c];
+                    }
                 // A column's reference is its maximum less kHead when it was set, and moves only when a score
                 // exceeds it by kMost. Weights 2^z thus reach from 2^kHead at the maximum up to 2^kMost, inside
                 // fp16's range, and keep 11 bits down to 2^-(14 + kHead) of the largest; below that the step is
@@ -573,9 +595,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                     // ---- V^T: rows are this lane's D/8 elements, columns keys 2t, 2t+1, 2t+8, 2t+9
                     const int r1 = 16 * (kSlabs * warp + b) + 2 * t;
                     const uint8_t *vp = stage + C::CODES + C::SCALES + r1 * (D / 2) + g * (D / 16);
-                    const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + r1 * GROUPS + g * GROUPS / 8;
+                    const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + r1 * GROUPS;
                     uint32_t v[4][VW];
-                    uint32_t sc[4];
+                    uint32_t sc[2];  // the scales of this lane's group for keys 2t, 2t+1 and 2t+8, 2t+9
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = (j & 1) + 8 * (j >> 1);
@@ -583,17 +605,25 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                             *reinterpret_cast<uint2 *>(v[j]) = *reinterpret_cast<const uint2 *>(vp + r * (D / 2));
                         else
                             v[j][0] = *reinterpret_cast<const uint32_t *>(vp + r * (D / 2));
-                        sc[j] = sp[r * GROUPS];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (GROUPS == 4) {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(sp + 8 * j * GROUPS);
+                            sc[j] = __byte_perm(w.x, w.y, pick);
+                        } else {
+                            sc[j] = __byte_perm(*reinterpret_cast<const uint32_t *>(sp + 8 * j * GROUPS), 0u, pick);
+                        }
                     }
                     if (!whole) {
                         // what an unseen slot holds may be any byte, a NaN scale among them: it becomes zero
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int key = key0 + 16 * b + 2 * t + (j & 1) + 8 * (j >> 1);
-                            if (key < span.lo || key >= span.hi) sc[j] = 0u;
+                            if (key < span.lo || key >= span.hi) sc[j >> 1] &= (j & 1) ? 0x00ffu : 0xff00u;
                         }
                     }
-                    const Dequant d0(scales2(sc[0], sc[1])), d1(scales2(sc[2], sc[3]));
+                    const Dequant d0(scales2(sc[0])), d1(scales2(sc[1]));
 #pragma unroll
                     for (int w = 0; w < VW; ++w)
 #pragma unroll
