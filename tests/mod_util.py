@@ -29,10 +29,13 @@ def attend(q, k, v, seen, lens, cap=0.0, slopes=None, p_half=2.0 ** -8, out=torc
     """64-bit attention and a bound on each element's error. q [B][Hq][Sq][D], k and v [B][Hkv][Sk][D] (any
     float type; exact values), seen [B][Sq][Sk]. The bound counts
       - P rounded to 1 / p_half steps: p_half * A, A = sum_j p_j |v_j|
-      - p_abs per key, where P's type has a smallest step (fp16: 2^-24). The 4-bit kernel's weights are
-        2^(z - m) with the largest at least 2^7 (m is a maximum less 7, and only ever replaced by a larger
-        one), so l >= 2^7 and half of that step is 2^-25 / 2^7 = 2^-32 of l; a merge of partials scales an
-        error by what it scales the partial's weights, and the partial with the largest m keeps l >= 2^7
+      - p_abs per key, where P's type has a smallest step (fp16: 2^-24). The 4-bit kernel rounds a weight
+        w = 2^(z - m) and then w * s, s the value's scale, each to fp16: 2^-11 of itself twice (p_half
+        2^-10), or half of the smallest step, 2^-25 (times s for the first). A value is q * s, |q| <= 8, and
+        l >= 2^4 (m is a maximum less 4, and only ever replaced by a larger one), so a key adds at most
+        2^-25 * 8 * (1 + s) / 2^4 = 2^-26 * (1 + s); s is at most a sixth of the largest |v| of its group
+        (a / 7 rounded to 4 bits). A merge of partials scales an error by what it scales the partial's
+        weights, and the partial with the largest m keeps l >= 2^4
       - scores: D products and D sums in 32 bits (2^-23 each on the tensor cores) of size |q||k|; scale,
         cap and bias a few roundings and the tanh fit (1e-6 relative in all); an error e of a score moves
         a weight by the factor 1 + e and the sum of weights by as much: 2 e A
@@ -79,5 +82,5 @@ def attend(q, k, v, seen, lens, cap=0.0, slopes=None, p_half=2.0 ** -8, out=torc
             A = p @ vv.abs()
             tol[b, h] = (p_half + 2 * e + 2.0 ** -17) * A + HALF[out] * o[b, h].abs() + 1e-30
             if p_abs:
-                tol[b, h] += p_abs * (sb.double() @ vv.abs())
+                tol[b, h] += p_abs * (sb.double() @ (1 + vv.abs().amax(1, keepdim=True)))
     return o, tol

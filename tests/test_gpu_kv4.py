@@ -273,7 +273,7 @@ def test_attention(cuda_dev, case):
     o, scr = run(q, pl, table, total, lens, P, ts.attn_mod(softcap=cap, causal=causal, slopes=sl), out, dev)
     assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
     seen = visible(B, Sq, lens, causal, Sk=k.shape[2], dev=dev)
-    ref, tol = attend(q, k, v, seen, lens, cap, sl, p_half=2.0 ** -11, p_abs=2.0 ** -32, out=out)
+    ref, tol = attend(q, k, v, seen, lens, cap, sl, p_half=2.0 ** -10, p_abs=2.0 ** -26, out=out)
     check(o, ref, tol, str(case))
     assert (o.transpose(1, 2)[~seen.any(2)] == 0).all()
 
@@ -303,7 +303,7 @@ def test_key_ranges(cuda_dev, Sq, D):
     q = torch.randn(B, Hq, Sq, D, generator=g, device=dev).bfloat16()
     o, scr = run(q, pl, table, total, lens, P, ts.attn_mod(causal=1, key_begin=begin, key_end=end), torch.float32, dev)
     assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
-    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -11, p_abs=2.0 ** -32)
+    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -10, p_abs=2.0 ** -26)
     check(o, ref, tol)
     assert (o.transpose(1, 2)[~seen.any(2)] == 0).all()
 
@@ -320,7 +320,7 @@ def test_rows_of_any_size(cuda_dev):
     q[0, 7] = 0
     o, _ = run(q, pl, table, total, lens, P, None, torch.float32, dev)
     seen = visible(1, 1, lens, 0, Sk=k.shape[2], dev=dev)
-    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -11, p_abs=2.0 ** -32)
+    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -10, p_abs=2.0 ** -26)
     check(o, ref, tol)
     q[0, 2, 0, 7] = float("nan")
     o2, _ = run(q, pl, table, total, lens, P, None, torch.float32, dev)
@@ -338,7 +338,7 @@ def test_bad_page_is_reported_and_later_calls_are_clean(cuda_dev):
     rc, code = ts.attn_flash_status(scr)
     assert rc == ts.ATTN_ERR_DEVICE and code == ts.ATTN_DEV_BAD_PAGE
     seen = visible(2, 1, lens, 0, Sk=k.shape[2], dev=dev)
-    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -11, p_abs=2.0 ** -32)
+    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -10, p_abs=2.0 ** -26)
     check(o[1], ref[1], tol[1], "the other sequence")
     o, _ = run(q, pl, table, total, lens, P, None, torch.float32, dev, scr)
     assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
@@ -412,7 +412,7 @@ def test_decode_steps_in_a_graph(cuda_dev):
     q = gb[0].view(B, Hq, 1, D)
     k, v = k.view(B, Hkv, Sk, D), v.view(B, Hkv, Sk, D)
     seen = visible(B, 1, n, 1, Sk=Sk, dev=dev)
-    ref, tol = attend(q, torch.nan_to_num(k), torch.nan_to_num(v), seen, n, 30.0, p_half=2.0 ** -11, p_abs=2.0 ** -32)
+    ref, tol = attend(q, torch.nan_to_num(k), torch.nan_to_num(v), seen, n, 30.0, p_half=2.0 ** -10, p_abs=2.0 ** -26)
     check(gb[1], ref, tol)
 
 

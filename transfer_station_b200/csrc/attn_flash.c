@@ -389,7 +389,8 @@ int attn_flash_kv4_stream(const uint16_t *Q, const uint8_t *K_codes, const uint8
     int rc = ts_paged_check(Q, K_codes, V_codes, block_table, seq_lens, O, B, Hq, Hkv, Sq, D, page_size, num_pages,
                             max_pages, scratch);
     if (rc == ATTN_ERR_ARGS) return rc;
-    if ((long long)page_size * max_pages > 0x7fffffffLL - 1024 || (long long)B * Hkv > 0x7fffffffLL) return ATTN_ERR_ARGS;
+    /* (the kernel looks a few tiles past the last key: its key indexes stay within 32 bits) */
+    if ((long long)page_size * max_pages > 0x7fffffffLL - 65536 || (long long)B * Hkv > 0x7fffffffLL) return ATTN_ERR_ARGS;
     fa_problem f;
     ts_fill(&f, Q, NULL, NULL, B * Hq, B * Hkv, Sq, max_pages * page_size, D, 0, 0);
     const int mrc = ts_set_mod(&f, mod, Hkv);

@@ -2,23 +2,30 @@
 // positions per sequence.
 //
 // What bounds it: the cache bytes, D/2 + D/32 per key and per value, read once (68 B at D = 128 against
-// 256 in bf16). At the measured copy rate an SM receives about 24 bytes, 46 elements, per clock, and
-// every element has to become a number for the tensor cores, so the arithmetic per element decides
-// whether the kernel keeps up:
-//   * Dequantisation is two instructions a pair: one LOP3 puts two nibbles under the fp16 exponent of
-//     1024 (1024 + n, or 1024 + 16 n for the high nibble of a byte), one HFMA2 by (s/16, -64.5 s) or
-//     (s/256, -4.5 s) gives (n - 8) s / 16 exactly: s has 4 significant bits, so 64.5 s and 4.5 s fit
-//     fp16's 11, and the product inside the FMA is not rounded. The factor 16 goes into the score's
-//     scale and the output's. fp16 rather than bf16: the weights P keep 11 bits, and Q, 8 bits wide, is
-//     exact after a power-of-two scale per row.
-//   * Keys are the M side of mma.m16n8k16 and the queries of a kv head the N side, so a group of up to 8
-//     query rows costs one MMA per 16 keys x 16 elements with no padding rows; P^T for the second product
-//     comes from the score fragment by two movmatrix transposes. tcgen05 would need the dequantised tile
-//     written to shared memory (2 bytes an element: 92 of the 128 bytes a clock) and 128 rows of queries
-//     or a TMEM round trip of the weights; here the elements never leave registers.
-//   * A lane's elements of a key are one contiguous run (D/4 of K, D/8 of V), so each key row is read from
-//     shared memory with one vector load a lane, and the k order inside the MMA is whatever the nibbles
-//     give: Q's fragments are permuted to match.
+// 256 in bf16). At the measured copy rate an SM receives about 24 bytes, 46 elements, per clock, and every
+// element has to reach the tensor cores as a number. What an SM sub-partition was measured to take: an
+// m16n8k16 fp16 MMA 8.2 cycles, a logic or fp16 instruction 2, and they overlap little (an MMA and four
+// LOPs: 13). So:
+//   * A nibble n under a mask is already a number: the fp16 subnormal n * 2^-24 (n * 2^-20 for the high
+//     nibble of a byte), two to an operand register by one LOP. MMAs take subnormals exactly, though the sum
+//     is then aligned as if they were normal and loses up to ten bits (24 of them remain, measured).
+//   * First product: the keys enter like that; the high nibbles' factor 16 is in Q's fragment. The offset 8
+//     and the scales stay off the elements: one accumulator per 32-element group gets -8 * 2^-24 *
+//     sum(Q over the group) added and is multiplied by the key's scale once. (e4m3 operands, whose
+//     nibbles need no more than a mask either and pair with Q split in two, ran at half this speed.)
+//   * Second product: one HFMA2 turns a masked pair into (n - 8) * 2^-9, normal numbers again, because the
+//     lost bits would not average out over long contexts. The value's scale goes into the weight, one
+//     fragment per group. (An MMA by -8 in place of the HFMA2s took 7% longer.)
+//   * ldmatrix gives each lane one 32-bit word of one group per key (K), and, transposed, two keys' same
+//     four elements in the halves of a register (V): the operand layouts without a permute. The code tiles
+//     come by TMA with the 64-byte (D = 64: 32-byte) swizzle, so the eight rows of a matrix lie in
+//     different banks.
+// Dequantising everything to fp16 with the scales took 131 us where this takes 129 us (B = 64,
+// Sk = 8192, 32/8 heads, D = 128; streaming the same bytes without arithmetic: 96).
+// Keys are the M side of mma.m16n8k16 and the query rows of a kv head the N side: up to 8 rows cost one
+// MMA per 16 keys x 16 elements, with no padding rows. tcgen05 would need the operand tile written back to
+// shared memory (2 bytes an element: 92 of the 128 bytes a clock) and 128 rows of queries. fp16 rather than
+// bf16: the weights keep 11 bits, and Q, 8 bits wide, is exact after a power-of-two scale per row.
 //
 // Work split. Tiles of kTile keys of all (sequence, kv head, row block) units form one list; CTA c of G
 // takes the c-th G-th of it, whatever the lengths are, so a ragged batch stays balanced without the host
@@ -26,6 +33,7 @@
 // One producer warp per CTA streams tiles into a ring of shared-memory stages with untiled bulk copies;
 // four consumer warps take 32 keys of each tile, each with its own running maximum and accumulator, merged
 // in shared memory at a unit's end.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -50,7 +58,7 @@ constexpr int kSlabs = 2;        // 16-key MMA rows of a warp and tile
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kMinTiles = 1;     // a CTA takes at least this many tiles (fewer CTAs work on small problems)
 
-constexpr float kHead = 7.f, kMost = 15.f;  // see the weights
+constexpr float kHead = 4.f, kMost = 7.f;  // see the weights
 
 struct Kv4Params {
     const uint16_t *Q;
@@ -75,19 +83,27 @@ struct Kv4Config {
     static constexpr int CODES = kTile * D / 2, SCALES = kTile * D / ATTN_KV4_GROUP;
     static constexpr int STAGE = 2 * (CODES + SCALES);
     static constexpr int NS = D == 128 ? 3 : 6;
+    static constexpr int V_CODES = CODES, K_SCALES = 2 * CODES, V_SCALES = 2 * CODES + SCALES;  // in a stage
     static constexpr int ROWS = 8 * NT;
     static constexpr int MERGE = kWarps * ROWS * (D + 4) * 4;  // one warp's accumulator rows, padded
     static constexpr int OFF_MERGE = NS * STAGE;
     static constexpr int OFF_ML = OFF_MERGE + MERGE;           // m, l [kWarps][ROWS]
     static constexpr int OFF_BAR = OFF_ML + 2 * kWarps * ROWS * 4;
-    static constexpr int SMEM = OFF_BAR + 2 * NS * 8;
+    static constexpr int SMEM = OFF_BAR + 2 * NS * 8 + 1024;  // + alignment of the swizzled tiles
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(  // (not volatile: a pure function of its operands, free to be scheduled)
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same from zero.
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -105,28 +121,32 @@ __device__ __forceinline__ __half2 scales2(uint32_t bytes) {
     return __half2(r);
 }
 
-// What turns the nibbles of a pair of scales into numbers: see the file's head.
-struct Dequant {
-    __half2 lo, lo_add, hi, hi_add;
-    __device__ __forceinline__ explicit Dequant(__half2 s)
-        : lo(__hmul2(s, __float2half2_rn(1.f / 16.f))),
-          lo_add(__hmul2(s, __float2half2_rn(-64.5f))),
-          hi(__hmul2(s, __float2half2_rn(1.f / 256.f))),
-          hi_add(__hmul2(s, __float2half2_rn(-4.5f))) {}
-    // (x & mask) | 1024's exponent in one LOP3: written out, the compiler emits two with an immediate each
-    __device__ __forceinline__ static uint32_t place(uint32_t x, uint32_t mask) {
-        uint32_t r;
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(0x64006400u));
-        return r;
-    }
-    // nibbles at bits 0 and 16, and at bits 4 and 20
-    __device__ __forceinline__ uint32_t low(uint32_t x) const {
-        return as_u32(__hfma2(as_half2(place(x, 0x000f000fu)), lo, lo_add));
-    }
-    __device__ __forceinline__ uint32_t high(uint32_t x) const {
-        return as_u32(__hfma2(as_half2(place(x, 0x00f000f0u)), hi, hi_add));
-    }
-};
+// Four 8x8 matrices of 16-bit elements; lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // fp16: n * 2^-24, n * 2^-20
+constexpr float kKeyUnit = 1.f / 16777216.f, kUnit = 1.f / 512.f;  // 2^-24 and 2^-9: what 1 stands for as a key, a value
+
+// A pair of masked nibbles -> (n - 8) * 2^-9, exact: times 2^15 (2^11), less 2^-6. (The constants as bits: the
+// conversion functions are not folded.)
+constexpr uint32_t kTwo15 = 0x78007800u, kTwo11 = 0x68006800u, kMinusEight = 0xa400a400u;
+__device__ __forceinline__ uint32_t centre_low(uint32_t x) {
+    return as_u32(__hfma2(as_half2(x & kLow), as_half2(kTwo15), as_half2(kMinusEight)));
+}
+__device__ __forceinline__ uint32_t centre_high(uint32_t x) {
+    return as_u32(__hfma2(as_half2(x & kHigh), as_half2(kTwo11), as_half2(kMinusEight)));
+}
 
 // A sequence: its keys, the span [lo, hi) outside which no query of it sees one, and the tiles of that
 // span (at least one, so that a sequence without keys gets its zero rows). The span is read from the key
@@ -255,15 +275,35 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// A slab's 16 rows of codes: lane (g, t) gets word t of every group of rows g and g + 8, or transposed the
+// 16-bit column g of every group of rows 2t, 2t + 1 and 2t + 8, 2t + 9. `off`: the lane's swizzled row.
+template <int D, bool TRANS>
+__device__ __forceinline__ void load_rows(uint32_t slab, uint32_t off, uint32_t (&r0)[D / 32], uint32_t (&r1)[D / 32]) {
+    auto load = [](uint32_t (&r)[4], uint32_t addr) {
+        if constexpr (TRANS)
+            ldmatrix4_trans(r, addr);
+        else
+            ldmatrix4(r, addr);
+    };
+    if constexpr (D == 128) {
+        load(r0, slab + off);
+        load(r1, slab + off + 8 * 64);
+    } else {
+        uint32_t r[4];
+        load(r, slab + off);
+        r0[0] = r[0], r0[1] = r[1], r1[0] = r[2], r1[1] = r[3];
+    }
+}
+
 // MOD: the call has a cap, a bias or key ranges.
 template <int D, int NT, bool MOD>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+    kv4_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Kv4Params p) {
     using C = Kv4Config<D, NT>;
-    constexpr int KW = D / 32;             // 32-bit words of a key row that a lane holds (its quarter of the row)
-    constexpr int VW = D / 64;             // words of a value row that a lane holds (its eighth)
     constexpr int MT = D / 16;             // 16-element tiles of the output
     constexpr int GROUPS = D / ATTN_KV4_GROUP;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ int abort_flag_s;
     volatile int *abort_flag = &abort_flag_s;
     const uint32_t base = smem_u32(smem), bars = base + C::OFF_BAR;
@@ -277,6 +317,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
             mbar_init(empty(s), kWarps);
         }
         fence_mbar_init();
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
     }
     pdl_wait();
     pdl_trigger();
@@ -330,12 +372,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 __syncwarp();
                 if (mine) {
                     const int row0 = (int)(((long long)(c0 + lane) * rows) % P);
-                    const size_t at = ((size_t)my_id * p.Hkv + kvh) * P + row0;  // row of the pools
+                    const int plane = my_id * p.Hkv + kvh;
+                    const size_t at = (size_t)plane * P + row0;  // row of the scale pools
                     const uint32_t dst = base + st * C::STAGE, bar = full(st);
-                    bulk_load(dst + lane * code_bytes, p.kc + at * (D / 2), code_bytes, bar);
-                    bulk_load(dst + C::CODES + lane * scale_bytes, p.ks + at * GROUPS, scale_bytes, bar);
-                    bulk_load(dst + C::CODES + C::SCALES + lane * code_bytes, p.vc + at * (D / 2), code_bytes, bar);
-                    bulk_load(dst + 2 * C::CODES + C::SCALES + lane * scale_bytes, p.vs + at * GROUPS, scale_bytes, bar);
+                    tma_load_3d(dst + lane * code_bytes, &tmK, bar, 0, row0, plane);
+                    bulk_load(dst + C::K_SCALES + lane * scale_bytes, p.ks + at * GROUPS, scale_bytes, bar);
+                    tma_load_3d(dst + C::V_CODES + lane * code_bytes, &tmV, bar, 0, row0, plane);
+                    bulk_load(dst + C::V_SCALES + lane * scale_bytes, p.vs + at * GROUPS, scale_bytes, bar);
                 }
                 __syncwarp();
                 if (++st == C::NS) {
@@ -367,9 +410,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
     float *ml = reinterpret_cast<float *>(smem + C::OFF_ML);
     const int rows_all = p.group * p.Sq;
     const bool has_cap = MOD && p.cap_out > 0.f, has_bias = MOD && p.slopes != nullptr;
-    // byte selector of a value group's scales for a pair of keys
-    const uint32_t pick = GROUPS == 4 ? (uint32_t)((g >> 1) | ((4 + (g >> 1)) << 4)) | 0x4400u
-                                      : (uint32_t)((g >> 2) | ((2 + (g >> 2)) << 4)) | 0x4400u;
+    // This lane's row and 16-byte chunk for ldmatrix, swizzled. D = 128: matrix m is chunk m of rows 0..7 (a
+    // second load takes rows 8..15); D = 64: chunk m % 2 of rows 8 (m / 2) ..
+    uint32_t rows_off;
+    if constexpr (D == 128) {
+        const int r = lane & 7, m = lane >> 3;
+        rows_off = r * 64 + ((m ^ ((r >> 1) & 3)) << 4);
+    } else {
+        const int r = (lane & 7) + 8 * (lane >> 4), m = (lane >> 3) & 1;
+        rows_off = r * 32 + ((m ^ ((r >> 2) & 1)) << 4);
+    }
     int st = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -381,46 +431,58 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
         const int row0 = rb * C::ROWS;
         const size_t qrow0 = ((size_t)b * p.Hkv + kvh) * rows_all + row0;  // row of Q and O
 
-        // ---- Q fragments: lane (g, t) holds query row g's quarter t, scaled by a power of two per row
-        uint32_t qf[NT][D / 16][2];
-        float fac[NT][2];  // raw score -> scaled score, for this lane's two query columns
+        // ---- Q fragments: lane (g, t) holds, of query row g, elements 8t..8t+7 of every group, scaled by a
+        // power of two per row
+        uint32_t qf[NT][GROUPS][4];
+        float start[NT][GROUPS][2];  // -8 * 2^-24 * sum of Q over a group, for this lane's two query columns
+        float fac[NT][2];            // accumulator -> scaled score, for the same
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const bool have = row0 + 8 * n + g < rows_all;
-            const uint16_t *src = p.Q + (qrow0 + 8 * n + g) * D + t * (D / 4);
-            uint32_t raw[D / 8];
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (have) v = *reinterpret_cast<const uint4 *>(src + 8 * w);
-                raw[4 * w] = v.x, raw[4 * w + 1] = v.y, raw[4 * w + 2] = v.z, raw[4 * w + 3] = v.w;
-            }
+            const uint16_t *src = p.Q + (qrow0 + 8 * n + g) * D + 8 * t;
+            uint32_t raw[GROUPS][4];
             float a = 0.f;
 #pragma unroll
-            for (int w = 0; w < D / 8; ++w)
-                a = fmaxf(a, fmaxf(fabsf(__uint_as_float(raw[w] << 16)), fabsf(__uint_as_float(raw[w] & 0xffff0000u))));
+            for (int w = 0; w < GROUPS; ++w) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (have) v = *reinterpret_cast<const uint4 *>(src + ATTN_KV4_GROUP * w);
+                raw[w][0] = v.x, raw[w][1] = v.y, raw[w][2] = v.z, raw[w][3] = v.w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    a = fmax3(a, fabsf(__uint_as_float(raw[w][i] << 16)), fabsf(__uint_as_float(raw[w][i] & 0xffff0000u)));
+            }
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-            // 2^-e with the row's largest magnitude in [1, 2) after it (a zero or non-finite row stays)
+            // 2^(4-e) puts the row's largest magnitude into [16, 32) (a zero or non-finite row stays)
             const int e = (int)(__float_as_uint(a) >> 23) - 127;
-            const bool plain = a == 0.f || e >= 128 || e <= -126;
-            const float down = plain ? 1.f : __uint_as_float((uint32_t)(127 - e) << 23);
-            const float up = plain ? 1.f : __uint_as_float((uint32_t)(127 + e) << 23);
-            // word w of a key row holds nibbles 0..7 = elements 8w..8w+7 in pairs (0,4) (1,5) (2,6) (3,7)
-            auto element = [&](int i) {
-                const uint32_t v = raw[i >> 1];
-                return __uint_as_float((i & 1) ? (v & 0xffff0000u) : (v << 16)) * down;
-            };
+            const bool plain = a == 0.f || e >= 128 || e <= -120;
+            const float down = plain ? 1.f : __uint_as_float((uint32_t)(131 - e) << 23);
+            const float up = plain ? 1.f : __uint_as_float((uint32_t)(123 + e) << 23);
 #pragma unroll
-            for (int w = 0; w < KW; ++w)
+            for (int w = 0; w < GROUPS; ++w) {
+                // a word's nibbles pair up as elements (0,4) (1,5) (2,6) (3,7); the odd pairs are high nibbles
+                auto element = [&](int i) {
+                    const uint32_t v = raw[w][i >> 1];
+                    return __uint_as_float((i & 1) ? (v & 0xffff0000u) : (v << 16)) * down;
+                };
+                float sum = 0.f;
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                    qf[n][2 * w + (h >> 1)][h & 1] =
-                        as_u32(__floats2half2_rn(element(8 * w + h), element(8 * w + h + 4)));
-            const float c0 = __shfl_sync(0xffffffffu, up, 8 * t), c1 = __shfl_sync(0xffffffffu, up, 8 * t + 4);
-            const float unit = 16.f * (has_cap ? p.cap_in : p.scale_log2);
-            fac[n][0] = c0 * unit;
-            fac[n][1] = c1 * unit;
+                for (int h = 0; h < 4; ++h) {
+                    const float part = (h & 1) ? 0.0625f : 1.f;
+                    const __half2 q = __floats2half2_rn(element(h) * part, element(h + 4) * part);
+                    qf[n][w][h] = as_u32(q);
+                    const float2 f = __half22float2(q);
+                    sum += (f.x + f.y) / part;
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= -8.f * kKeyUnit;
+                start[n][w][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                start[n][w][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            }
+            const float unit = (has_cap ? p.cap_in : p.scale_log2) / kKeyUnit;
+            fac[n][0] = __shfl_sync(0xffffffffu, up, 8 * t) * unit;
+            fac[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * unit;
         }
         // ---- this lane's query columns: keys seen, position, bias
         int lo[NT][2], hi[NT][2], pos[NT][2], near[NT][2];
@@ -465,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 if (!ok) break;
             }
             const uint8_t *stage = smem + st * C::STAGE;
+            const uint32_t stage_at = base + st * C::STAGE;
             const int key0 = (span.t0 + i) * kTile + 16 * kSlabs * warp;  // this warp's keys
             if (key0 < span.hi && key0 + 16 * kSlabs > span.lo) {
                 // ---- S^T = K Q^T
@@ -473,30 +536,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 for (int b = 0; b < kSlabs; ++b) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
-                    const int r0 = 16 * (kSlabs * warp + b) + g;
-                    const uint8_t *rowp = stage + r0 * (D / 2) + t * (D / 8);
-                    uint32_t ka[KW], kb[KW];
-                    if constexpr (KW == 4) {
-                        *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(rowp);
-                        *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(rowp + 8 * (D / 2));
+                    const int r0 = 16 * (kSlabs * warp + b);  // the slab's first row in the stage
+                    uint32_t k0[GROUPS], k1[GROUPS];          // this lane's word of every group, keys g and g + 8
+                    load_rows<D, false>(stage_at + r0 * (D / 2), rows_off, k0, k1);
+                    const uint8_t *sp = stage + C::K_SCALES + (r0 + g) * GROUPS;
+                    float2 f0[GROUPS / 2], f1[GROUPS / 2];    // their scales
+                    if constexpr (GROUPS == 4) {
+                        const uint32_t w0 = *reinterpret_cast<const uint32_t *>(sp);
+                        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(sp + 8 * GROUPS);
+                        f0[0] = __half22float2(scales2(w0 & 0xffffu)), f0[1] = __half22float2(scales2(w0 >> 16));
+                        f1[0] = __half22float2(scales2(w1 & 0xffffu)), f1[1] = __half22float2(scales2(w1 >> 16));
                     } else {
-                        *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(rowp);
-                        *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(rowp + 8 * (D / 2));
+                        f0[0] = __half22float2(scales2(*reinterpret_cast<const uint16_t *>(sp)));
+                        f1[0] = __half22float2(scales2(*reinterpret_cast<const uint16_t *>(sp + 8 * GROUPS)));
                     }
-                    const uint8_t *sp = stage + C::CODES + r0 * GROUPS + t * GROUPS / 4;
-                    const __half2 sc = scales2(sp[0] | ((uint32_t)sp[8 * GROUPS] << 8));
-                    const Dequant da(__low2half2(sc)), db(__high2half2(sc));
+                    float d[GROUPS][NT][4];
 #pragma unroll
-                    for (int w = 0; w < KW; ++w) {
-                        uint32_t x = ka[w], y = kb[w];
-                        uint32_t a[4] = {da.low(x), db.low(y), da.high(x), db.high(y)};
+                    for (int w = 0; w < GROUPS; ++w) {
+                        const uint32_t xs = k0[w] >> 8, ys = k1[w] >> 8;
+                        const uint32_t a0[4] = {k0[w] & kLow, k1[w] & kLow, k0[w] & kHigh, k1[w] & kHigh};
+                        const uint32_t a1[4] = {xs & kLow, ys & kLow, xs & kHigh, ys & kHigh};
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816(s[b][n], a, qf[n][2 * w][0], qf[n][2 * w][1]);
-                        x >>= 8;
-                        y >>= 8;
-                        a[0] = da.low(x), a[1] = db.low(y), a[2] = da.high(x), a[3] = db.high(y);
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816_zero(d[w][n], a0, qf[n][w][0], qf[n][w][1]);
+                            mma16816(d[w][n], a1, qf[n][w][2], qf[n][w][3]);
+                        }
+                    }
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816(s[b][n], a, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                    for (int w = 0; w < GROUPS; ++w) {
+                        const float c0 = (w & 1) ? f0[w >> 1].y : f0[w >> 1].x, c1 = (w & 1) ? f1[w >> 1].y : f1[w >> 1].x;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            s[b][n][0] = fmaf(d[w][n][0] + start[n][w][0], c0, s[b][n][0]);
+                            s[b][n][1] = fmaf(d[w][n][1] + start[n][w][1], c0, s[b][n][1]);
+                            s[b][n][2] = fmaf(d[w][n][2] + start[n][w][0], c1, s[b][n][2]);
+                            s[b][n][3] = fmaf(d[w][n][3] + start[n][w][1], c1, s[b][n][3]);
+                        }
                     }
                 }
                 // ---- scores less their column's reference, log2 units: element e is key g + 8 (e / 2) of its
@@ -544,9 +619,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                         above |= mx > most[n][c];
                     }
                 // A column's reference is its maximum less kHead when it was set, and moves only when a score
-                // exceeds it by kMost. Weights 2^z thus reach from 2^kHead at the maximum up to 2^kMost, inside
-                // fp16's range, and keep 11 bits down to 2^-(14 + kHead) of the largest; below that the step is
-                // 2^-(24 + kHead) of it. (Until a column has seen a key, most is -inf and the reference 0.)
+                // exceeds it by kMost: weights reach from 2^kHead at the maximum up to 2^kMost, which times
+                // the largest scale (448) still is an fp16 number. (Until a column has seen a key, most is
+                // -inf and the reference 0.)
                 if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -592,27 +667,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                         pf[n][0] = transpose8x8(as_u32(__floats2half2_rn(w[0], w[1])));
                         pf[n][1] = transpose8x8(as_u32(__floats2half2_rn(w[2], w[3])));
                     }
-                    // ---- V^T: rows are this lane's D/8 elements, columns keys 2t, 2t+1, 2t+8, 2t+9
-                    const int r1 = 16 * (kSlabs * warp + b) + 2 * t;
-                    const uint8_t *vp = stage + C::CODES + C::SCALES + r1 * (D / 2) + g * (D / 16);
-                    const uint8_t *sp = stage + 2 * C::CODES + C::SCALES + r1 * GROUPS;
-                    uint32_t v[4][VW];
-                    uint32_t sc[2];  // the scales of this lane's group for keys 2t, 2t+1 and 2t+8, 2t+9
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = (j & 1) + 8 * (j >> 1);
-                        if constexpr (VW == 2)
-                            *reinterpret_cast<uint2 *>(v[j]) = *reinterpret_cast<const uint2 *>(vp + r * (D / 2));
-                        else
-                            v[j][0] = *reinterpret_cast<const uint32_t *>(vp + r * (D / 2));
-                    }
+                    // ---- V^T: lane (g, t) holds elements 4g..4g+3 of every group for keys 2t, 2t+1 and 2t+8, 2t+9
+                    const int r0 = 16 * (kSlabs * warp + b);
+                    uint32_t v0[GROUPS], v1[GROUPS];
+                    load_rows<D, true>(stage_at + C::V_CODES + r0 * (D / 2), rows_off, v0, v1);
+                    // the keys' scales, pairs of keys side by side: sc[half][..] bytes (A0 B0 A1 B1) (A2 B2 A3 B3)
+                    const uint8_t *sp = stage + C::V_SCALES + (r0 + 2 * t) * GROUPS;
+                    uint32_t sc[2][GROUPS / 2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         if constexpr (GROUPS == 4) {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(sp + 8 * j * GROUPS);
-                            sc[j] = __byte_perm(w.x, w.y, pick);
+                            uint2 w = *reinterpret_cast<const uint2 *>(sp + 8 * j * GROUPS);
+                            sc[j][0] = __byte_perm(w.x, w.y, 0x5140);
+                            sc[j][1] = __byte_perm(w.x, w.y, 0x7362);
                         } else {
-                            sc[j] = __byte_perm(*reinterpret_cast<const uint32_t *>(sp + 8 * j * GROUPS), 0u, pick);
+                            sc[j][0] = __byte_perm(*reinterpret_cast<const uint32_t *>(sp + 8 * j * GROUPS), 0u, 0x3120);
                         }
                     }
                     if (!whole) {
@@ -620,27 +689,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int key = key0 + 16 * b + 2 * t + (j & 1) + 8 * (j >> 1);
-                            if (key < span.lo || key >= span.hi) sc[j >> 1] &= (j & 1) ? 0x00ffu : 0xff00u;
+                            if (key < span.lo || key >= span.hi)
+#pragma unroll
+                                for (int w = 0; w < GROUPS / 2; ++w) sc[j >> 1][w] &= (j & 1) ? 0x00ff00ffu : 0xff00ff00u;
                         }
                     }
-                    const Dequant d0(scales2(sc[0])), d1(scales2(sc[1]));
 #pragma unroll
-                    for (int w = 0; w < VW; ++w)
+                    for (int w = 0; w < GROUPS; ++w) {
+                        const uint32_t x = v0[w], y = v1[w], xs = x >> 8, ys = y >> 8;
+                        const uint32_t a0[4] = {centre_low(x), centre_high(x), centre_low(y), centre_high(y)};
+                        const uint32_t a1[4] = {centre_low(xs), centre_high(xs), centre_low(ys), centre_high(ys)};
+                        const __half2 s0 = scales2((w & 1) ? sc[0][w >> 1] >> 16 : sc[0][w >> 1] & 0xffffu);
+                        const __half2 s1 = scales2((w & 1) ? sc[1][w >> 1] >> 16 : sc[1][w >> 1] & 0xffffu);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            // the same half word of both keys: nibble n of each half is element 8w + 4h + n
-                            uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
-                            uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
-                            uint32_t a[4] = {d0.low(x), d0.high(x), d1.low(y), d1.high(y)};
-                            const int i0 = 4 * w + 2 * h;
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) mma16816(acc[n][i0], a, pf[n][0], pf[n][1]);
-                            x >>= 8;
-                            y >>= 8;
-                            a[0] = d0.low(x), a[1] = d0.high(x), a[2] = d1.low(y), a[3] = d1.high(y);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) mma16816(acc[n][i0 + 1], a, pf[n][0], pf[n][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            const uint32_t p0 = as_u32(__hmul2(as_half2(pf[n][0]), s0));
+                            const uint32_t p1 = as_u32(__hmul2(as_half2(pf[n][1]), s1));
+                            mma16816(acc[n][2 * w], a0, p0, p1);
+                            mma16816(acc[n][2 * w + 1], a1, p0, p1);
                         }
+                    }
                 }
             }
             __syncwarp();
@@ -652,8 +720,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
         }
 
         // ---- merge the four warps: rows [ROWS] x D
-        // lane (g, t) holds, for query columns 2t and 2t+1, the D/8 consecutive elements from g * D/8
-#pragma unroll
+        #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -664,11 +731,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                     ml[warp * C::ROWS + 8 * n + 2 * t + c] = most[n][c] == -INFINITY ? -INFINITY : ref[n][c];
                     ml[(kWarps + warp) * C::ROWS + 8 * n + 2 * t + c] = l[n][c];
                 }
-                float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (D + 4) + g * (D / 8);
+                // elements 4g..4g+3 of every group
+                float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (D + 4) + 4 * g;
 #pragma unroll
-                for (int i = 0; i < MT; i += 2)
-                    *reinterpret_cast<float4 *>(dst + 2 * i) = make_float4(acc[n][i][c], acc[n][i][c + 2],
-                                                                          acc[n][i + 1][c], acc[n][i + 1][c + 2]);
+                for (int w = 0; w < GROUPS; ++w)
+                    *reinterpret_cast<float4 *>(dst + ATTN_KV4_GROUP * w) =
+                        make_float4(acc[n][2 * w][c], acc[n][2 * w][c + 2], acc[n][2 * w + 1][c],
+                                    acc[n][2 * w + 1][c + 2]);
             }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
         const bool cut = begin > 0 || end < nt;
@@ -705,8 +774,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_kernel(const Kv
                 }
                 *reinterpret_cast<float4 *>(p.part_acc + (slot + r) * D + 4 * c4) = o;
             } else if (row0 + r < rows_all) {
-                // V carries s/16
-                const float inv = L > 0.f ? 16.f / L : (L == 0.f ? 0.f : L);
+                const float inv = L > 0.f ? 1.f / (kUnit * L) : (L == 0.f ? 0.f : L);
                 const size_t at = (qrow0 + r) * D + 4 * c4;
                 if (p.o_bf16)
                     *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.O) + at) =
@@ -785,12 +853,37 @@ __global__ void __launch_bounds__(128) kv4_combine(const Kv4Params p) {
         L = fmaf(f, sl[w], L);
         o = fmaf(f, sacc[w][col], o);
     }
-    const float inv = L > 0.f ? 16.f / L : (L == 0.f ? 0.f : L);
+    const float inv = L > 0.f ? 1.f / (kUnit * L) : (L == 0.f ? 0.f : L);
     const size_t at = (((size_t)b * p.Hkv + kvh) * rows_all + row) * D + col;
     if (p.o_bf16)
         reinterpret_cast<uint16_t *>(p.O)[at] = (uint16_t)pack_bf16x2(o * inv, 0.f);
     else
         reinterpret_cast<float *>(p.O)[at] = o * inv;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A code pool as {D/2 bytes, rows of a page, page x kv head}, boxes of one page's rows up to a tile.
+bool make_code_map(CUtensorMap *m, const uint8_t *codes, const ts_kv4_problem *P, int D) {
+    static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<EncodeTiledFn>(ptr);
+        return nullptr;
+    }();
+    if (!fn) return false;
+    const cuuint64_t row = (cuuint64_t)D / 2, ps = (cuuint64_t)P->page_size;
+    cuuint64_t dims[3] = {row, ps, (cuuint64_t)P->num_pages * P->Hkv};
+    cuuint64_t strides[2] = {row, row * ps};
+    cuuint32_t box[3] = {(cuuint32_t)row, (cuuint32_t)(ps < kTile ? ps : kTile), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(codes), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename... KArgs, typename... Args>
@@ -866,7 +959,9 @@ int run(const ts_kv4_problem *P, cudaStream_t st) {
     const size_t acc = (size_t)2 * ctas * 8 * NT * D;
     if (acc * 4 + (size_t)units * sizeof(int2) > (size_t)P->part_rows * D * 4) return ATTN_ERR_ARGS;
     p.desc = reinterpret_cast<int2 *>(P->part_acc + acc);
-    const int rc = launch(kv4_kernel<D, NT, MOD>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, p);
+    CUtensorMap tmK, tmV;
+    if (!make_code_map(&tmK, P->k_codes, P, D) || !make_code_map(&tmV, P->v_codes, P, D)) return ATTN_ERR_CUDA;
+    const int rc = launch(kv4_kernel<D, NT, MOD>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, tmK, tmV, p);
     if (rc != ATTN_OK) return rc;
     return launch(kv4_combine<D, NT>, dim3((unsigned)units, 8 * NT), dim3(128), 0, st, p);
 }
