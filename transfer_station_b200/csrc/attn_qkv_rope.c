@@ -138,7 +138,9 @@ int attn_qkv_rope_kv4_stream(const uint16_t *qkv, const int *positions, const fl
     P.page_size = page_size;
     P.num_pages = num_pages;
     P.max_pages = max_pages;
-    return ts_rope_run(&P, stream);
+    if (ts_cc_major() != 10) return ATTN_ERR_NOT_SM100;
+    if (P.n_vec <= 0) return ts_clear_status(P.status, stream);
+    return ts_launch_kv4_append(&P, stream);
 }
 
 int attn_kv4_unpack_stream(const uint8_t *K_codes, const uint8_t *K_scales, const uint8_t *V_codes,
@@ -169,7 +171,6 @@ int attn_kv4_unpack_stream(const uint8_t *K_codes, const uint8_t *K_scales, cons
     P.num_pages = num_pages;
     P.max_pages = max_pages;
     P.status = (int *)scratch;
-    rc = ts_clear_status(P.status, stream);
-    if (rc != ATTN_OK) return rc;
+    if (B == 0 || S == 0) return ts_clear_status(P.status, stream);
     return ts_launch_kv4_unpack(&P, stream);
 }

@@ -127,8 +127,8 @@ typedef struct ts_rope_problem {
 
 int ts_launch_qkv_rope(const ts_rope_problem *p, void *stream);
 
-/* The 4-bit cache (attn_kv4.h): its tokens as bf16 (kv4_cache.cu), and attention over it
- * (kv4_attn.cu). */
+/* The 4-bit cache (attn_kv4.h): its producer and its tokens as bf16 (kv4_cache.cu), and attention
+ * over it (kv4_attn.cu). */
 typedef struct ts_kv4_problem {
     const uint16_t *Q;
     const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
@@ -146,6 +146,7 @@ typedef struct ts_kv4_problem {
 } ts_kv4_problem;
 
 int ts_launch_kv4(const ts_kv4_problem *p, void *stream);
+int ts_launch_kv4_append(const ts_rope_problem *p, void *stream);
 int ts_launch_kv4_unpack(const ts_kv4_problem *p, void *stream);
 int ts_launch_rope_table(float *cos_sin, int max_pos, int rot, double theta, void *stream);
 

@@ -20,13 +20,11 @@
 // A lane owns both members of each pair it rotates -- for the rotate-half form elements
 // [8li, 8li+8) and [rot/2 + 8li, +8), for the interleaved form 16 consecutive elements -- so the
 // rotation needs no shuffle; only the norm's sum of squares crosses lanes (log2(D/16) shuffles).
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <atomic>
 
-#include "attn_kv4.h"
 #include "attn_qkv_rope.h"
 #include "fa_launch.h"
 #include "sm100_ptx.cuh"
@@ -130,37 +128,8 @@ __device__ __forceinline__ void lane_chunks(const ts_rope_problem &a, int li, in
     }
 }
 
-// KV4: a key or value row goes to the 4-bit pools instead. The lane's 16 consecutive elements (one half of a
-// group; the lanes of a group are neighbours) become a nibble each under the group's scale.
-template <int D>
-__device__ __forceinline__ void store_kv4(uint4 ra, uint4 rb, uint8_t *codes, uint8_t *scales, long long row, int li,
-                                          bool write) {
-    float x[16];
-    unpack8(ra, x);
-    unpack8(rb, x + 8);
-    float m = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));  // (a NaN leaves m as it is)
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    const __nv_fp8_storage_t s8 = __nv_cvt_float_to_fp8(m / 7.0f, __NV_SATFINITE, __NV_E4M3);
-    const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(s8, __NV_E4M3)));
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        // the quotient is rounded to fp32 first: it has at most 12 significant bits next to a tie, so
-        // the second rounding sees the tie or the right side of it
-        const float q = x[e] / s;
-        const int n = q == q ? (int)fminf(fmaxf(rintf(q), -8.f), 7.f) : 0;
-        w[e >> 3] |= (uint32_t)((s > 0.f ? n : 0) + 8) << (4 * (e & 7));
-    }
-    if (write) {
-        *reinterpret_cast<uint2 *>(codes + row * (D / 2) + 8 * li) = make_uint2(w[0], w[1]);
-        if ((li & 1) == 0) scales[row * (D / ATTN_KV4_GROUP) + (li >> 1)] = s8;
-    }
-}
-
-template <int D, bool NEOX, bool PAGED, bool KV4 = false>
-__global__ void __maxnreg__(KV4 ? 80 : 72) qkv_rope_kernel(ts_rope_problem a) {
+template <int D, bool NEOX, bool PAGED>
+__global__ void __maxnreg__(72) qkv_rope_kernel(ts_rope_problem a) {
     constexpr int G = D / 16;                        // lanes per head vector, 16 elements each
     constexpr int CV = kRopeChunk / (D * 2);         // head vectors per stage
     constexpr int NG = kRopeConsumerWarps * 32 / G;  // lane groups of the consumers
@@ -247,13 +216,13 @@ __global__ void __maxnreg__(KV4 ? 80 : 72) qkv_rope_kernel(ts_rope_problem a) {
         const int st = (int)(k % kRopeStages);
         if (!mbar_wait(full0 + 8 * st, (uint32_t)(k / kRopeStages) & 1u, &abort_flag, a.status, kDevErrTimeoutKV))
             break;
-        uint8_t *stage = smem + st * kRopeChunk + (size_t)grp * (D * 2);
+        const uint8_t *stage = smem + st * kRopeChunk + (size_t)grp * (D * 2);
         const long long vbase = c * CV + grp;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const uint4 raj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + oa * 2);
             const uint4 rbj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + ob * 2);
-            if (!KV4 && j == PER - 1) {  // the stage's last bytes are in registers: release it
+            if (j == PER - 1) {  // the stage's last bytes are in registers: release it
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty0 + 8 * st);
             }
@@ -270,21 +239,8 @@ __global__ void __maxnreg__(KV4 ? 80 : 72) qkv_rope_kernel(ts_rope_problem a) {
             for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
             for (int o = G / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o, G);
-            float root = 0.f;
-            if constexpr (KV4) {
-                // A last bit of the root can move a code by one: the k heads' is summed in double and
-                // rounded once, whatever the order.
-                if (__any_sync(FULL, kind == 1 && has_kn)) {
-                    double sd = 0.0;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sd = fma((double)x[e], (double)x[e], sd);
-#pragma unroll
-                    for (int o = G / 2; o >= 1; o >>= 1) sd += __shfl_xor_sync(FULL, sd, o, G);
-                    root = (float)rsqrt(sd * (1.0 / D) + (double)a.eps);
-                }
-            }
             if (kind == 0 ? has_qn : (kind == 1 && has_kn)) {
-                const float r = KV4 && kind == 1 ? root : rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
+                const float r = rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
                 const float *w = kind == 0 ? wq : wk;
                 float wv[16];
                 *reinterpret_cast<float4 *>(wv) = *reinterpret_cast<const float4 *>(w + oa);
@@ -311,34 +267,7 @@ __global__ void __maxnreg__(KV4 ? 80 : 72) qkv_rope_kernel(ts_rope_problem a) {
                     }
                 }
             }
-            if constexpr (KV4) {
-                // the rotated row goes through its own slot of the stage, so that a lane gets 16
-                // consecutive elements of one group whatever the pairing was
-                uint8_t *vec = stage + (size_t)j * NG * (D * 2);
-                if (act && kind == 1) {
-                    *reinterpret_cast<uint4 *>(vec + oa * 2) = pack8(x);
-                    *reinterpret_cast<uint4 *>(vec + ob * 2) = pack8(x + 8);
-                }
-                __syncwarp();
-                if (__any_sync(FULL, act && kind > 0)) {
-                    const uint4 la = *reinterpret_cast<const uint4 *>(vec + 32 * li);
-                    const uint4 lb = *reinterpret_cast<const uint4 *>(vec + 32 * li + 16);
-                    const long long off = T.kv_off + (h - (kind == 1 ? a.Hq : a.Hq + a.Hkv)) * T.kv_stride;
-                    store_kv4<D>(la, lb, kind == 1 ? a.k_codes : a.v_codes, kind == 1 ? a.k_scales : a.v_scales, off / D,
-                                 li, act && T.ok && kind > 0);
-                }
-                if (j == PER - 1) {  // the stage is done with; its rows were written: order them before the
-                                     // next bulk copy into it
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(empty0 + 8 * st);
-                }
-                if (act && T.ok && kind == 0) {
-                    uint16_t *dst = T.q_base + h * T.q_stride;
-                    *reinterpret_cast<uint4 *>(dst + oa) = pack8(x);
-                    *reinterpret_cast<uint4 *>(dst + ob) = pack8(x + 8);
-                }
-            } else if (act && T.ok) {
+            if (act && T.ok) {
                 uint16_t *dst = kind == 0   ? T.q_base + h * T.q_stride
                                 : kind == 1 ? a.K + T.kv_off + (h - a.Hq) * T.kv_stride
                                             : a.V + T.kv_off + (h - a.Hq - a.Hkv) * T.kv_stride;
@@ -376,10 +305,10 @@ __global__ void rope_table_kernel(float *cs, int max_pos, int rot, double theta)
 
 // Once per device and kernel instance: opt in to the ring's shared memory and read how many CTAs
 // fit on an SM (0: not set up yet). Concurrent first calls both do the same work.
-template <int D, bool NEOX, bool PAGED, bool KV4 = false>
+template <int D, bool NEOX, bool PAGED>
 static int rope_resident() {
     static std::atomic<int> resident[64];
-    auto kern = ts::qkv_rope_kernel<D, NEOX, PAGED, KV4>;
+    auto kern = ts::qkv_rope_kernel<D, NEOX, PAGED>;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return -1;
     const bool cached = dev >= 0 && dev < 64;
@@ -400,9 +329,6 @@ static int rope_resident() {
 template <int D>
 static int pick_rope_resident(const ts_rope_problem *p) {
     const bool neox = p->style == ATTN_ROPE_NEOX, paged = p->block_table != nullptr;
-    if constexpr (D <= 128) {
-        if (p->k_codes) return neox ? rope_resident<D, true, true, true>() : rope_resident<D, false, true, true>();
-    }
     if (neox) return paged ? rope_resident<D, true, true>() : rope_resident<D, true, false>();
     return paged ? rope_resident<D, false, true>() : rope_resident<D, false, false>();
 }
@@ -410,9 +336,6 @@ static int pick_rope_resident(const ts_rope_problem *p) {
 template <int D>
 static void (*pick_rope_kernel(const ts_rope_problem *p))(ts_rope_problem) {
     const bool neox = p->style == ATTN_ROPE_NEOX, paged = p->block_table != nullptr;
-    if constexpr (D <= 128) {
-        if (p->k_codes) return neox ? ts::qkv_rope_kernel<D, true, true, true> : ts::qkv_rope_kernel<D, false, true, true>;
-    }
     if (neox) return paged ? ts::qkv_rope_kernel<D, true, true> : ts::qkv_rope_kernel<D, true, false>;
     return paged ? ts::qkv_rope_kernel<D, false, true> : ts::qkv_rope_kernel<D, false, false>;
 }
