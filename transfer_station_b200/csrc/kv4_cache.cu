@@ -98,21 +98,16 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 __device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf16x2(v.x, v.y); }
-// Two integers saturated to [-8, 7] in the low byte (the second lowest), the rest moved up.
-__device__ __forceinline__ uint32_t pack_s4(int hi, int lo, uint32_t rest) {
-    uint32_t d;
-    asm("cvt.pack.sat.s4.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(hi), "r"(lo), "r"(rest));
-    return d;
-}
-
 // 16 consecutive bf16 elements, half of a group (the other half is the neighbouring lane's) -> nibbles and
 // the group's scale s.
 //
 // The quotient x / s has to be rounded as the quotient, ties to even, and ties do occur (x has 8 bits, s has
 // 4). y = x * (1/s) is off by at most one step of fp32; one correction by the exact residual x - y s (a step
 // of Newton's iteration, as Markstein used it) lands on the tie when there is one, and never on one that is
-// not there: next to a tie, x / s differs from it by 2^-12 at least. Adding 1.5 * 2^23 rounds it. Groups with
-// a NaN, an infinity or a scale at the end of its range take the plain way below.
+// not there: next to a tie, x / s differs from it by 2^-12 at least. Adding 1.5 * 2^23 + 8 rounds it and leaves
+// q + 8 in the low bits; eight of them, each times a power of 16, make a word once the constant's share is
+// taken off. |x / s| <= 7.5, so nothing saturates, unless s is subnormal. Groups with a NaN, an infinity or a
+// saturated scale take the plain way below.
 __device__ __forceinline__ uint2 quantise(uint4 ra, uint4 rb, __nv_fp8_storage_t &s8) {
     const uint32_t r[8] = {ra.x, ra.y, ra.z, ra.w, rb.x, rb.y, rb.z, rb.w};
     uint32_t m2 = 0u;  // magnitudes order as their bits: largest of the even and of the odd elements
@@ -125,19 +120,24 @@ __device__ __forceinline__ uint2 quantise(uint4 ra, uint4 rb, __nv_fp8_storage_t
         s8 = __nv_cvt_float_to_fp8(__uint_as_float(m << 16) / 7.0f, __NV_SATFINITE, __NV_E4M3);
         const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(s8, __NV_E4M3)));
         const float inv = s > 0.f ? 1.0f / s : 0.f;  // a scale of zero: every quotient is zero
-        const float2 inv2 = make_float2(inv, inv), s2 = make_float2(-s, -s), magic = make_float2(12582912.f, 12582912.f);
+        const float2 inv2 = make_float2(inv, inv), s2 = make_float2(-s, -s), magic = make_float2(12582920.f, 12582920.f);
+        const bool small = s < 0.015625f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            w[h] = 0u;
+            uint32_t t[8];
 #pragma unroll
-            for (int e = 3; e >= 0; --e) {
+            for (int e = 0; e < 4; ++e) {
                 const float2 x = unpack2(r[4 * h + e]);
                 const float2 y = __fmul2_rn(x, inv2);
-                const float2 q = __ffma2_rn(__ffma2_rn(y, s2, x), inv2, y);
-                const float2 t = __fadd2_rn(q, magic);
-                w[h] = pack_s4(__float_as_int(t.y) - 0x4b400000, __float_as_int(t.x) - 0x4b400000, w[h]);
+                float2 q = __ffma2_rn(__ffma2_rn(y, s2, x), inv2, y);
+                if (small) q = make_float2(fminf(fmaxf(q.x, -8.f), 7.f), fminf(fmaxf(q.y, -8.f), 7.f));
+                q = __fadd2_rn(q, magic);
+                t[2 * e] = __float_as_uint(q.x), t[2 * e + 1] = __float_as_uint(q.y);
             }
-            w[h] ^= 0x88888888u;  // two's complement -> q + 8
+            w[h] = t[7];
+#pragma unroll
+            for (int e = 6; e >= 0; --e) w[h] = w[h] * 16u + t[e];
+            w[h] -= 0x4b400000u * 0x11111111u;
         }
     } else {
         float a = 0.f;
@@ -164,10 +164,13 @@ __device__ __forceinline__ uint2 quantise(uint4 ra, uint4 rb, __nv_fp8_storage_t
     return make_uint2(w[0], w[1]);
 }
 
-// |x| of a bf16 value held in fp32, as a double, by moving bits: zero and subnormals come out below 2^-126,
-// which a sum of squares does not see.
-__device__ __forceinline__ double magnitude(float x) {
-    return __hiloint2double((int)(((__float_as_uint(x) & 0x7fffffffu) >> 3) + 0x38000000u), 0);
+// |x| of the lower and the upper bf16 of a word as doubles, by moving bits: zero and subnormals come out below
+// 2^-126, which a sum of squares does not see.
+__device__ __forceinline__ double magnitude_lo(uint32_t w) {
+    return __hiloint2double((int)((w & 0x7fffu) * 8192u + 0x38000000u), 0);
+}
+__device__ __forceinline__ double magnitude_hi(uint32_t w) {
+    return __hiloint2double((int)(((w & 0x7fff0000u) >> 3) + 0x38000000u), 0);
 }
 
 // parts: how many items a token's head vectors are divided into. zero: (-0, -0), see the rotation.
@@ -196,28 +199,33 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
     const int heads = a.Hq + 2 * a.Hkv, q_passes = (a.Hq + VPW - 1) / VPW, kv_passes = (a.Hkv + VPW - 1) / VPW;
     const int passes = q_passes + 2 * kv_passes, share = (passes + parts - 1) / parts;
     uint16_t *mine = cross[warp] + grp * D;
-    const long long items = (long long)tokens * parts, step = (long long)(gridDim.x - 1) * kAppendWarps;
-    for (long long item = (long long)(blockIdx.x - 1) * kAppendWarps + warp; item < items; item += step) {
-        const int tok = (int)(item / parts), part = (int)(item - (long long)tok * parts);
+    // (parts > 1 only when there are few tokens: the items fit 32 bits)
+    const unsigned items = (unsigned)tokens * (unsigned)parts, step = (gridDim.x - 1) * kAppendWarps;
+    for (unsigned item = (blockIdx.x - 1) * kAppendWarps + warp; item < items; item += step) {
+        const int tok = parts == 1 ? (int)item : (int)(item / (unsigned)parts), part = (int)(item - (unsigned)tok * parts);
         const int first = part * share, last = min(passes, first + share);
         if (first >= last) continue;
         const uint16_t *src = a.qkv + (long long)tok * heads * D;
-        // A pass takes VPW heads of one kind (0 q, 1 k, 2 v); head of this lane's group within its kind.
-        auto kind_of = [&](int pass) { return pass < q_passes ? 0 : (pass < q_passes + kv_passes ? 1 : 2); };
-        auto head_of = [&](int pass, int kind) {
-            return (pass - (kind == 0 ? 0 : (kind == 1 ? q_passes : q_passes + kv_passes))) * VPW + grp;
+        // A pass takes VPW heads of one kind (0 q, 1 k, 2 v). Where the next load is: kind, head of this lane's
+        // group within the kind, offset of its vector in the token's row, passes left of the kind.
+        int nkind, nhead, noff, nleft;
+        auto seek = [&](int pass) {
+            nkind = pass < q_passes ? 0 : (pass < q_passes + kv_passes ? 1 : 2);
+            const int from = nkind == 0 ? 0 : (nkind == 1 ? q_passes : q_passes + kv_passes);
+            nhead = (pass - from) * VPW + grp;
+            noff = (nhead + (nkind == 0 ? 0 : (nkind == 1 ? a.Hq : a.Hq + a.Hkv))) * D;
+            nleft = from + (nkind == 0 ? q_passes : kv_passes) - pass;
         };
-        auto fetch = [&](int pass, uint4 &x, uint4 &y) {
-            const int kind = kind_of(pass), h = head_of(pass, kind);
-            if (h < (kind == 0 ? a.Hq : a.Hkv)) {
-                const uint16_t *at = src + (h + (kind == 0 ? 0 : (kind == 1 ? a.Hq : a.Hq + a.Hkv))) * D;
+        auto fetch = [&](uint4 &x, uint4 &y) {
+            if (nhead < (nkind == 0 ? a.Hq : a.Hkv)) {
                 // (a value row is not rotated: 16 consecutive elements, as the quantiser wants them)
-                x = *reinterpret_cast<const uint4 *>(at + (kind == 2 ? 16 * li : oa));
-                y = *reinterpret_cast<const uint4 *>(at + (kind == 2 ? 16 * li + 8 : ob));
+                x = *reinterpret_cast<const uint4 *>(src + noff + (nkind == 2 ? 16 * li : oa));
+                y = *reinterpret_cast<const uint4 *>(src + noff + (nkind == 2 ? 16 * li + 8 : ob));
             }
         };
         uint4 na = make_uint4(0u, 0u, 0u, 0u), nb = na;
-        fetch(first, na, nb);
+        seek(first);
+        fetch(na, nb);
         const int pos = ld_plan(a.positions + tok);
         const int b = tok / a.S, sq = tok - b * a.S;
         const Slot slot = find_slot(a.block_table, b, pos, a.page_size, a.max_pages, a.num_pages);
@@ -249,7 +257,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
                     double sd = 0.0;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const double u = magnitude(x[e].x), v = magnitude(x[e].y);
+                        const uint32_t word = (&ra.x)[e & 3], other = (&rb.x)[e & 3];
+                        const double u = magnitude_lo(e < 4 ? word : other), v = magnitude_hi(e < 4 ? word : other);
                         sd = fma(v, v, fma(u, u, sd));
                     }
 #pragma unroll
@@ -304,18 +313,30 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
             oa4 = make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
             ob4 = make_uint4(pack2(x[4]), pack2(x[5]), pack2(x[6]), pack2(x[7]));
         };
+        const long long q_step = (long long)VPW * a.S * D, kv_step = (long long)VPW * a.page_size;
+        uint16_t *q_at = q_row + (long long)nhead * a.S * D;  // (of a q pass)
+        long long row = row0 + (long long)nhead * a.page_size;  // (of a k or v pass)
         for (int pass = first; pass < last; ++pass) {
             const uint4 ra = na, rb = nb;
-            if (pass + 1 < last) fetch(pass + 1, na, nb);
-            const int kind = kind_of(pass), h = head_of(pass, kind);  // the kind is the warp's
+            const int kind = nkind, h = nhead;  // the kind is the warp's
+            if (pass + 1 < last) {
+                if (--nleft == 0) {
+                    seek(pass + 1);
+                } else {
+                    nhead += VPW;
+                    noff += VPW * D;
+                }
+                fetch(na, nb);
+            }
             if (kind == 0) {
                 uint4 oa4, ob4;
                 rotated(std::false_type{}, ra, rb, oa4, ob4);
                 if (h < a.Hq) {
-                    uint16_t *dst = q_row + (long long)h * a.S * D;
-                    *reinterpret_cast<uint4 *>(dst + oa) = oa4;
-                    *reinterpret_cast<uint4 *>(dst + ob) = ob4;
+                    *reinterpret_cast<uint4 *>(q_at + oa) = oa4;
+                    *reinterpret_cast<uint4 *>(q_at + ob) = ob4;
                 }
+                q_at += q_step;
+                if (nkind != 0) row = row0 + (long long)grp * a.page_size;
             } else {
                 uint4 la = ra, lb = rb;
                 if (kind == 1) {
@@ -331,11 +352,11 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
                 __nv_fp8_storage_t s8;
                 const uint2 w = quantise(la, lb, s8);
                 if (h < a.Hkv) {
-                    const long long row = row0 + (long long)h * a.page_size;
                     uint8_t *codes = kind == 1 ? a.k_codes : a.v_codes, *scales = kind == 1 ? a.k_scales : a.v_scales;
                     *reinterpret_cast<uint2 *>(codes + row * (D / 2) + 8 * li) = w;
                     if ((li & 1) == 0) scales[row * (D / ATTN_KV4_GROUP) + (li >> 1)] = s8;
                 }
+                row = nkind == kind ? row + kv_step : row0 + (long long)grp * a.page_size;
             }
         }
     }
