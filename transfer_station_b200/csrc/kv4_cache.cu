@@ -1,12 +1,13 @@
 // kv4_cache.cu -- writing and reading back the 4-bit paged key cache (attn_kv4.h): the QKV producer that
 // appends to it, and its tokens as contiguous bf16 K and V. Byte work; HBM is the floor of both.
 //
-// Producer. A warp takes a token (or, when there are few, a part of its heads) and walks its head vectors
-// 32 / (D / 16) at a time, 16 elements a lane, with the next vectors' loads in flight; what depends on the
-// token alone (slot, cos and sin of the lane's frequencies) is loaded once a token. The arithmetic is
-// attn_qkv_rope_paged_stream's, operation by operation, in packed fp32 pairs. Measured: a variant of that
-// call's kernel (bulk copies into a ring, a lane group per vector) ran 5,760 warp instructions a token of
-// 48 heads and was bound by them; this one runs APPEND_INST.
+// Producer. A warp takes a token (or, when there are few, a part of its heads) and walks its q, k and v heads
+// 32 / (D / 16) at a time, 16 elements a lane. The loads run four passes ahead through a ring in the warp's
+// shared memory; what depends on the token alone (slot, cos and sin of the lane's frequencies) is loaded once a
+// token. The arithmetic is attn_qkv_rope_paged_stream's, operation by operation, in packed fp32 pairs. It is
+// bound by instruction issue: a variant of that call's kernel (bulk copies into a ring, a lane group per
+// vector) ran 5,760 warp instructions a token of 32 + 2 * 8 heads of 128, this one 2,970; the norm and the
+// rotation are template parameters, as branches of every pass they cost 10%. 16,384 such tokens: 79 us, 330 MB.
 //
 // A lane owns both members of each pair it rotates (rotate-half: elements [8i, 8i+8) and [rot/2 + 8i, +8);
 // interleaved: 16 consecutive), as in qkv_rope.cu. A rotated key then crosses through the warp's shared
@@ -34,7 +35,18 @@ namespace {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kDepth = 4;  // passes whose loads are in flight
 constexpr unsigned kFull = 0xffffffffu;
+
+// 16 bytes from global to shared memory, asynchronously; groups complete in the order of their commits.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // Row of token position `pos` of sequence b in the pools' planes (page * Hkv, row in the page), or why not.
 struct Slot {
@@ -173,12 +185,14 @@ __device__ __forceinline__ double magnitude_hi(uint32_t w) {
     return __hiloint2double((int)(((w & 0x7fff0000u) >> 3) + 0x38000000u), 0);
 }
 
-// parts: how many items a token's head vectors are divided into. zero: (-0, -0), see the rotation.
-template <int D, bool NEOX>
+// parts: how many items a token's head vectors are divided into. WHOLE: every element is rotated (rot == D).
+// NORM: 1 q heads, 2 k heads, 3 both. zero: (-0, -0), see the rotation.
+template <int D, bool NEOX, bool WHOLE, int NORM>
 __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_rope_problem a, int parts, float2 zero) {
     constexpr int G = D / 16, VPW = 32 / G;  // lanes of a vector, vectors of a warp's pass
     __shared__ __align__(16) uint16_t cross[kAppendWarps][VPW * D];
     __shared__ __align__(16) float wq[D], wk[D];
+    __shared__ __align__(16) uint8_t loads[kAppendWarps][kDepth * 1024];
     pdl_wait();
     pdl_trigger();
     const int tokens = a.B * a.S;
@@ -187,51 +201,165 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
         return;
     }
     for (int e = threadIdx.x; e < D; e += blockDim.x) {
-        wq[e] = a.q_norm_w ? __uint_as_float((uint32_t)a.q_norm_w[e] << 16) : 1.f;
-        wk[e] = a.k_norm_w ? __uint_as_float((uint32_t)a.k_norm_w[e] << 16) : 1.f;
+        if (NORM & 1) wq[e] = __uint_as_float((uint32_t)a.q_norm_w[e] << 16);
+        if (NORM & 2) wk[e] = __uint_as_float((uint32_t)a.k_norm_w[e] << 16);
     }
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % G, grp = lane / G;
     // the lane's two runs of 8 elements
-    const bool rot_lane = NEOX ? li < (a.rot >> 4) : 16 * li < a.rot;
+    const bool rot_lane = WHOLE || (NEOX ? li < (a.rot >> 4) : 16 * li < a.rot);
     const int oa = NEOX ? (rot_lane ? 8 * li : a.rot + 16 * (li - (a.rot >> 4))) : 16 * li;
     const int ob = NEOX && rot_lane ? (a.rot >> 1) + 8 * li : oa + 8;
     const int heads = a.Hq + 2 * a.Hkv, q_passes = (a.Hq + VPW - 1) / VPW, kv_passes = (a.Hkv + VPW - 1) / VPW;
-    const int passes = q_passes + 2 * kv_passes, share = (passes + parts - 1) / parts;
+    const int k_end = q_passes + kv_passes, passes = k_end + kv_passes, share = (passes + parts - 1) / parts;
     uint16_t *mine = cross[warp] + grp * D;
     // (parts > 1 only when there are few tokens: the items fit 32 bits)
     const unsigned items = (unsigned)tokens * (unsigned)parts, step = (gridDim.x - 1) * kAppendWarps;
-    for (unsigned item = (blockIdx.x - 1) * kAppendWarps + warp; item < items; item += step) {
-        const int tok = parts == 1 ? (int)item : (int)(item / (unsigned)parts), part = (int)(item - (unsigned)tok * parts);
-        const int first = part * share, last = min(passes, first + share);
-        if (first >= last) continue;
-        const uint16_t *src = a.qkv + (long long)tok * heads * D;
-        // A pass takes VPW heads of one kind (0 q, 1 k, 2 v). Where the next load is: kind, head of this lane's
-        // group within the kind, offset of its vector in the token's row, passes left of the kind.
-        int nkind, nhead, noff, nleft;
-        auto seek = [&](int pass) {
-            nkind = pass < q_passes ? 0 : (pass < q_passes + kv_passes ? 1 : 2);
-            const int from = nkind == 0 ? 0 : (nkind == 1 ? q_passes : q_passes + kv_passes);
-            nhead = (pass - from) * VPW + grp;
-            noff = (nhead + (nkind == 0 ? 0 : (nkind == 1 ? a.Hq : a.Hq + a.Hkv))) * D;
-            nleft = from + (nkind == 0 ? q_passes : kv_passes) - pass;
-        };
-        auto fetch = [&](uint4 &x, uint4 &y) {
-            if (nhead < (nkind == 0 ? a.Hq : a.Hkv)) {
-                // (a value row is not rotated: 16 consecutive elements, as the quantiser wants them)
-                x = *reinterpret_cast<const uint4 *>(src + noff + (nkind == 2 ? 16 * li : oa));
-                y = *reinterpret_cast<const uint4 *>(src + noff + (nkind == 2 ? 16 * li + 8 : ob));
+    const unsigned item0 = (blockIdx.x - 1) * kAppendWarps + warp;
+    auto token_of = [&](unsigned item) { return parts == 1 ? (int)item : (int)(item / (unsigned)parts); };
+    // Loads run kDepth passes ahead of the arithmetic, over the ends of items: every lane copies its own 32
+    // bytes of a pass into its own place of the warp's ring. A pass takes VPW heads of one kind (q, k, v). Where
+    // the next load is: item, pass, head of this lane's group within its kind and how many the kind has, the
+    // two runs' offsets in the token's row, passes left until the kind or the item changes.
+    unsigned nitem = item0;
+    int npass = 0, nlast = 0, nhead = 0, nheads = 0, na = 0, nb = 0, nleft = 0;
+    const uint16_t *nsrc = a.qkv;
+    auto seek = [&]() {
+        const int kind = npass < q_passes ? 0 : (npass < k_end ? 1 : 2);
+        const int from = kind == 0 ? 0 : (kind == 1 ? q_passes : k_end);
+        nhead = (npass - from) * VPW + grp;
+        nheads = kind == 0 ? a.Hq : a.Hkv;
+        const int off = (nhead + (kind == 0 ? 0 : (kind == 1 ? a.Hq : a.Hq + a.Hkv))) * D;
+        // (a value row is not rotated: 16 consecutive elements, as the quantiser wants them)
+        na = off + (kind == 2 ? 16 * li : oa);
+        nb = off + (kind == 2 ? 16 * li + 8 : ob);
+        const int end = min(nlast, kind == 0 ? q_passes : (kind == 1 ? k_end : passes));
+        nleft = end - npass;
+        npass = end;  // (the pass after the run)
+    };
+    auto next_run = [&]() {  // the next run of passes of one kind; an item without a pass is stepped over
+        if (npass >= nlast) {
+            for (nitem += nlast > 0 ? step : 0; nitem < items; nitem += step) {
+                const int tok = token_of(nitem);
+                npass = (int)(nitem - (unsigned)tok * parts) * share;
+                nlast = min(passes, npass + share);
+                nsrc = a.qkv + (long long)tok * heads * D;
+                if (npass < nlast) break;
             }
-        };
-        uint4 na = make_uint4(0u, 0u, 0u, 0u), nb = na;
-        seek(first);
-        fetch(na, nb);
+            if (nitem >= items) {
+                nleft = 0x7fffffff;
+                nheads = 0;  // nothing more is loaded
+                return;
+            }
+        }
+        seek();
+    };
+    const uint32_t ring = smem_u32(loads[warp]) + lane * 16;
+    auto fetch = [&](int stage) {
+        if (nhead < nheads) {
+            copy16(ring + stage * 1024, nsrc + na);
+            copy16(ring + stage * 1024 + 512, nsrc + nb);
+        }
+        copy_commit();
+        if (--nleft == 0) {
+            next_run();
+        } else {
+            nhead += VPW;
+            na += VPW * D;
+            nb += VPW * D;
+        }
+    };
+    next_run();
+    for (int st = 0; st < kDepth; ++st) fetch(st);
+    int stage = 0;
+    auto take = [&](uint4 &ra, uint4 &rb) {  // this pass's elements; its place takes the load kDepth passes on
+        copy_wait<kDepth - 1>();
+        ra = *reinterpret_cast<const uint4 *>(loads[warp] + stage * 1024 + lane * 16);
+        rb = *reinterpret_cast<const uint4 *>(loads[warp] + stage * 1024 + lane * 16 + 512);
+        fetch(stage);
+        stage = (stage + 1) % kDepth;
+    };
+    float2 c[4], sn[4];
+    // One pass over rotated heads (keys or queries): normed, rotated, rounded to bf16.
+    auto rotated = [&](auto key_tag, uint4 ra, uint4 rb, uint4 &oa4, uint4 &ob4) {
+        constexpr bool kKey = decltype(key_tag)::value;
+        float2 x[8] = {unpack2(ra.x), unpack2(ra.y), unpack2(ra.z), unpack2(ra.w),
+                       unpack2(rb.x), unpack2(rb.y), unpack2(rb.z), unpack2(rb.w)};
+        if constexpr ((NORM & (kKey ? 2 : 1)) != 0) {
+            float root;
+            if (kKey) {
+                // A last bit of the root can move a code by one: the k heads' sum is taken in double and the
+                // root rounded once, whatever the order.
+                const uint32_t w[8] = {ra.x, ra.y, ra.z, ra.w, rb.x, rb.y, rb.z, rb.w};
+                double sd = 0.0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double u = magnitude_lo(w[e]), v = magnitude_hi(w[e]);
+                    sd = fma(v, v, fma(u, u, sd));
+                }
+#pragma unroll
+                for (int o = G / 2; o >= 1; o >>= 1) sd += __shfl_xor_sync(kFull, sd, o, G);
+                // 1 / sqrt(v): the fp32 root, and one step of Newton's iteration in double
+                const double v = sd * (1.0 / D) + (double)a.eps;
+                const double r0 = (double)rsqrtf((float)v);
+                const double r1 = fma(0.5 * r0, fma(-v * r0, r0, 1.0), r0);
+                root = v > 1e-30 && v < 1e30 ? (float)r1 : (float)rsqrt(v);
+            } else {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(x[e].y, x[e].y, fmaf(x[e].x, x[e].x, ss));
+#pragma unroll
+                for (int o = G / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o, G);
+                root = rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
+            }
+            const float *w = kKey ? wk : wq;
+            const float2 r2 = make_float2(root, root);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float4 u = *reinterpret_cast<const float4 *>(w + oa + 2 * e);
+                const float4 v = *reinterpret_cast<const float4 *>(w + ob + 2 * e);
+                x[e] = __fmul2_rn(__fmul2_rn(x[e], r2), make_float2(u.x, u.y));
+                x[e + 1] = __fmul2_rn(__fmul2_rn(x[e + 1], r2), make_float2(u.z, u.w));
+                x[4 + e] = __fmul2_rn(__fmul2_rn(x[4 + e], r2), make_float2(v.x, v.y));
+                x[5 + e] = __fmul2_rn(__fmul2_rn(x[5 + e], r2), make_float2(v.z, v.w));
+            }
+        }
+        if (rot_lane) {
+            // Each product is rounded, then their sum: products as FMAs with a zero that the compiler does not
+            // know (it would fuse a packed product with the packed sum after it, whatever the intrinsics say),
+            // differences as FMAs by -1.
+            const float2 minus = make_float2(-1.f, -1.f);
+            if (NEOX) {  // pairs (x[e], x[4 + e]) at frequencies 8 li + 2e, + 1
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 u = x[e], w = x[4 + e];
+                    x[e] = __ffma2_rn(__ffma2_rn(w, sn[e], zero), minus, __ffma2_rn(u, c[e], zero));
+                    x[4 + e] = __fadd2_rn(__ffma2_rn(w, c[e], zero), __ffma2_rn(u, sn[e], zero));
+                }
+            } else {  // pairs (x[e].x, x[e].y) at frequency 8 li + e
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float u = x[e].x, w = x[e].y;
+                    const float cf = (e & 1) ? c[e >> 1].y : c[e >> 1].x, sf = (e & 1) ? sn[e >> 1].y : sn[e >> 1].x;
+                    x[e].x = __fsub_rn(__fmul_rn(u, cf), __fmul_rn(w, sf));
+                    x[e].y = __fadd_rn(__fmul_rn(w, cf), __fmul_rn(u, sf));
+                }
+            }
+        }
+        oa4 = make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
+        ob4 = make_uint4(pack2(x[4]), pack2(x[5]), pack2(x[6]), pack2(x[7]));
+    };
+    for (unsigned item = item0; item < items; item += step) {
+        const int tok = token_of(item), first = (int)(item - (unsigned)tok * parts) * share, last = min(passes, first + share);
+        if (first >= last) continue;
         const int pos = ld_plan(a.positions + tok);
         const int b = tok / a.S, sq = tok - b * a.S;
         const Slot slot = find_slot(a.block_table, b, pos, a.page_size, a.max_pages, a.num_pages);
-        const bool ok = slot.code == 0 && pos < a.max_pos;
-        if (!ok) continue;  // skipped whole (the status CTA reports it)
-        float2 c[4], sn[4];
+        uint4 ra, rb, oa4, ob4;
+        if (slot.code != 0 || pos >= a.max_pos) {  // skipped whole (the status CTA reports it)
+            for (int pass = first; pass < last; ++pass) take(ra, rb);
+            continue;
+        }
         if (rot_lane) {
             const float *row = a.cos_sin + (long long)pos * a.rot + 8 * li, *srow = row + (a.rot >> 1);
 #pragma unroll
@@ -242,122 +370,44 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
                 sn[2 * i] = make_float2(sv.x, sv.y), sn[2 * i + 1] = make_float2(sv.z, sv.w);
             }
         }
-        uint16_t *q_row = a.Q + ((long long)b * a.Hq * a.S + sq) * D;
-        const long long row0 = (long long)slot.page * a.Hkv * a.page_size + slot.row;
-        // One pass over rotated heads (K: keys, into the cache; else queries).
-        auto rotated = [&](auto key_tag, uint4 ra, uint4 rb, uint4 &oa4, uint4 &ob4) {
-            constexpr bool kKey = decltype(key_tag)::value;
-            float2 x[8] = {unpack2(ra.x), unpack2(ra.y), unpack2(ra.z), unpack2(ra.w),
-                           unpack2(rb.x), unpack2(rb.y), unpack2(rb.z), unpack2(rb.w)};
-            if (kKey ? a.k_norm_w != nullptr : a.q_norm_w != nullptr) {
-                float root;
-                if (kKey) {
-                    // A last bit of the root can move a code by one: the k heads' sum is taken in double and
-                    // the root rounded once, whatever the order.
-                    double sd = 0.0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t word = (&ra.x)[e & 3], other = (&rb.x)[e & 3];
-                        const double u = magnitude_lo(e < 4 ? word : other), v = magnitude_hi(e < 4 ? word : other);
-                        sd = fma(v, v, fma(u, u, sd));
-                    }
-#pragma unroll
-                    for (int o = G / 2; o >= 1; o >>= 1) sd += __shfl_xor_sync(kFull, sd, o, G);
-                    // 1 / sqrt(v): the fp32 root, and one step of Newton's iteration in double
-                    const double v = sd * (1.0 / D) + (double)a.eps;
-                    const double r0 = (double)rsqrtf((float)v);
-                    const double r1 = fma(0.5 * r0, fma(-v * r0, r0, 1.0), r0);
-                    root = v > 1e-30 && v < 1e30 ? (float)r1 : (float)rsqrt(v);
-                } else {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ss = fmaf(x[e].y, x[e].y, fmaf(x[e].x, x[e].x, ss));
-#pragma unroll
-                    for (int o = G / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o, G);
-                    root = rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
-                }
-                const float *w = kKey ? wk : wq;
-                const float2 r2 = make_float2(root, root);
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float4 u = *reinterpret_cast<const float4 *>(w + oa + 2 * e);
-                    const float4 v = *reinterpret_cast<const float4 *>(w + ob + 2 * e);
-                    x[e] = __fmul2_rn(__fmul2_rn(x[e], r2), make_float2(u.x, u.y));
-                    x[e + 1] = __fmul2_rn(__fmul2_rn(x[e + 1], r2), make_float2(u.z, u.w));
-                    x[4 + e] = __fmul2_rn(__fmul2_rn(x[4 + e], r2), make_float2(v.x, v.y));
-                    x[5 + e] = __fmul2_rn(__fmul2_rn(x[5 + e], r2), make_float2(v.z, v.w));
-                }
-            }
-            if (rot_lane) {
-                // Each product is rounded, then their sum: products as FMAs with a zero that the compiler does
-                // not know (it would fuse a packed product with the packed sum after it, whatever the
-                // intrinsics say), differences as FMAs by -1.
-                const float2 minus = make_float2(-1.f, -1.f);
-                if (NEOX) {  // pairs (x[e], x[4 + e]) at frequencies 8 li + 2e, + 1
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 u = x[e], w = x[4 + e];
-                        x[e] = __ffma2_rn(__ffma2_rn(w, sn[e], zero), minus, __ffma2_rn(u, c[e], zero));
-                        x[4 + e] = __fadd2_rn(__ffma2_rn(w, c[e], zero), __ffma2_rn(u, sn[e], zero));
-                    }
-                } else {  // pairs (x[e].x, x[e].y) at frequency 8 li + e
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float u = x[e].x, w = x[e].y;
-                        const float cf = (e & 1) ? c[e >> 1].y : c[e >> 1].x, sf = (e & 1) ? sn[e >> 1].y : sn[e >> 1].x;
-                        x[e].x = __fsub_rn(__fmul_rn(u, cf), __fmul_rn(w, sf));
-                        x[e].y = __fadd_rn(__fmul_rn(w, cf), __fmul_rn(u, sf));
-                    }
-                }
-            }
-            oa4 = make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
-            ob4 = make_uint4(pack2(x[4]), pack2(x[5]), pack2(x[6]), pack2(x[7]));
-        };
-        const long long q_step = (long long)VPW * a.S * D, kv_step = (long long)VPW * a.page_size;
-        uint16_t *q_at = q_row + (long long)nhead * a.S * D;  // (of a q pass)
-        long long row = row0 + (long long)nhead * a.page_size;  // (of a k or v pass)
-        for (int pass = first; pass < last; ++pass) {
-            const uint4 ra = na, rb = nb;
-            const int kind = nkind, h = nhead;  // the kind is the warp's
-            if (pass + 1 < last) {
-                if (--nleft == 0) {
-                    seek(pass + 1);
-                } else {
-                    nhead += VPW;
-                    noff += VPW * D;
-                }
-                fetch(na, nb);
-            }
-            if (kind == 0) {
-                uint4 oa4, ob4;
+        int pass = first;
+        if (pass < q_passes) {
+            int h = pass * VPW + grp;
+            uint16_t *at = a.Q + (((long long)b * a.Hq + h) * a.S + sq) * D;
+            const long long at_step = (long long)VPW * a.S * D;
+            for (const int end = min(last, q_passes); pass < end; ++pass, h += VPW, at += at_step) {
+                take(ra, rb);
                 rotated(std::false_type{}, ra, rb, oa4, ob4);
                 if (h < a.Hq) {
-                    *reinterpret_cast<uint4 *>(q_at + oa) = oa4;
-                    *reinterpret_cast<uint4 *>(q_at + ob) = ob4;
+                    *reinterpret_cast<uint4 *>(at + oa) = oa4;
+                    *reinterpret_cast<uint4 *>(at + ob) = ob4;
                 }
-                q_at += q_step;
-                if (nkind != 0) row = row0 + (long long)grp * a.page_size;
-            } else {
-                uint4 la = ra, lb = rb;
-                if (kind == 1) {
-                    uint4 oa4, ob4;
-                    rotated(std::true_type{}, ra, rb, oa4, ob4);
-                    *reinterpret_cast<uint4 *>(mine + oa) = oa4;
-                    *reinterpret_cast<uint4 *>(mine + ob) = ob4;
-                    __syncwarp();
-                    la = *reinterpret_cast<const uint4 *>(mine + 16 * li);
-                    lb = *reinterpret_cast<const uint4 *>(mine + 16 * li + 8);
-                    __syncwarp();
-                }
-                __nv_fp8_storage_t s8;
-                const uint2 w = quantise(la, lb, s8);
-                if (h < a.Hkv) {
-                    uint8_t *codes = kind == 1 ? a.k_codes : a.v_codes, *scales = kind == 1 ? a.k_scales : a.v_scales;
-                    *reinterpret_cast<uint2 *>(codes + row * (D / 2) + 8 * li) = w;
-                    if ((li & 1) == 0) scales[row * (D / ATTN_KV4_GROUP) + (li >> 1)] = s8;
-                }
-                row = nkind == kind ? row + kv_step : row0 + (long long)grp * a.page_size;
             }
+        }
+        const long long row0 = (long long)slot.page * a.Hkv * a.page_size + slot.row;
+        auto store = [&](uint4 x, uint4 y, int h, uint8_t *codes, uint8_t *scales) {
+            __nv_fp8_storage_t s8;
+            const uint2 w = quantise(x, y, s8);
+            if (h < a.Hkv) {
+                const long long row = row0 + (long long)h * a.page_size;
+                *reinterpret_cast<uint2 *>(codes + row * (D / 2) + 8 * li) = w;
+                if ((li & 1) == 0) scales[row * (D / ATTN_KV4_GROUP) + (li >> 1)] = s8;
+            }
+        };
+        for (const int end = min(last, k_end); pass < end; ++pass) {
+            take(ra, rb);
+            rotated(std::true_type{}, ra, rb, oa4, ob4);
+            *reinterpret_cast<uint4 *>(mine + oa) = oa4;
+            *reinterpret_cast<uint4 *>(mine + ob) = ob4;
+            __syncwarp();
+            ra = *reinterpret_cast<const uint4 *>(mine + 16 * li);
+            rb = *reinterpret_cast<const uint4 *>(mine + 16 * li + 8);
+            __syncwarp();
+            store(ra, rb, (pass - q_passes) * VPW + grp, a.k_codes, a.k_scales);
+        }
+        for (; pass < last; ++pass) {
+            take(ra, rb);
+            store(ra, rb, (pass - k_end) * VPW + grp, a.v_codes, a.v_scales);
         }
     }
 }
@@ -451,7 +501,7 @@ int launch(void (*kern)(KArgs...), dim3 grid, int threads, cudaStream_t st, Args
     return ATTN_OK;
 }
 
-template <int D, bool NEOX>
+template <int D, bool NEOX, bool WHOLE, int NORM>
 int launch_append(const ts_rope_problem *P, cudaStream_t st) {
     constexpr int VPW = 32 / (D / 16);
     const long long tokens = (long long)P->B * P->S, wave = (long long)ts_num_sms() * 3 * kAppendWarps;
@@ -460,8 +510,25 @@ int launch_append(const ts_rope_problem *P, cudaStream_t st) {
     long long parts = (wave + tokens - 1) / tokens;
     if (parts > passes) parts = passes;
     const long long ctas = (tokens * parts + kAppendWarps - 1) / kAppendWarps, most = (long long)ts_num_sms() * 3;
-    return launch(kv4_append_kernel<D, NEOX>, dim3((unsigned)((ctas < most ? ctas : most) + 1)), kAppendThreads, st, *P,
-                  (int)parts, make_float2(-0.f, -0.f));
+    return launch(kv4_append_kernel<D, NEOX, WHOLE, NORM>, dim3((unsigned)((ctas < most ? ctas : most) + 1)), kAppendThreads,
+                  st, *P, (int)parts, make_float2(-0.f, -0.f));
+}
+
+template <int D, bool NEOX, bool WHOLE>
+int launch_append(const ts_rope_problem *P, cudaStream_t st) {
+    switch ((P->q_norm_w ? 1 : 0) + (P->k_norm_w ? 2 : 0)) {
+    case 0: return launch_append<D, NEOX, WHOLE, 0>(P, st);
+    case 1: return launch_append<D, NEOX, WHOLE, 1>(P, st);
+    case 2: return launch_append<D, NEOX, WHOLE, 2>(P, st);
+    default: return launch_append<D, NEOX, WHOLE, 3>(P, st);
+    }
+}
+
+template <int D>
+int launch_append(const ts_rope_problem *P, cudaStream_t st) {
+    const bool neox = P->style == ATTN_ROPE_NEOX, whole = P->rot == D;
+    if (neox) return whole ? launch_append<D, true, true>(P, st) : launch_append<D, true, false>(P, st);
+    return whole ? launch_append<D, false, true>(P, st) : launch_append<D, false, false>(P, st);
 }
 
 template <int D>
@@ -483,9 +550,7 @@ int launch_unpack(const ts_kv4_problem *P, cudaStream_t st) {
 
 extern "C" int ts_launch_kv4_append(const ts_rope_problem *P, void *stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool neox = P->style == ATTN_ROPE_NEOX;
-    if (P->D == 64) return neox ? ts::launch_append<64, true>(P, st) : ts::launch_append<64, false>(P, st);
-    return neox ? ts::launch_append<128, true>(P, st) : ts::launch_append<128, false>(P, st);
+    return P->D == 64 ? ts::launch_append<64>(P, st) : ts::launch_append<128>(P, st);
 }
 
 extern "C" int ts_launch_kv4_unpack(const ts_kv4_problem *P, void *stream) {
