@@ -30,7 +30,7 @@ CC = os.environ.get("CC", "gcc")
 CC_FLAGS = ["-O2", "-std=c11", "-fPIC", "-Wall", "-Wextra"]
 
 CU_SOURCES = ["fa_fwd_sm100.cu", "fa_aux.cu", "fa_noalloc.cu", "fa_diag.cu", "fa_peer.cu", "qkv_rope.cu", "fa_mod.cu",
-              "kv4_attn.cu", "kv4_cache.cu",
+              "fa_rows.cu", "kv4_attn.cu", "kv4_cache.cu",
               "fa_mod_range.cu", "fa_mod_cap.cu", "fa_mod_bias.cu", "fa_mod_capbias.cu"]
 C_SOURCES = ["attn_flash.c", "attn_qkv_rope.c"]
 

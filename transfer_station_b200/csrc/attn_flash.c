@@ -322,6 +322,15 @@ static int ts_set_mod(fa_problem *p, const attn_mod *mod, int Hkv) {
 /* Runs a problem with modified scores. The bounds of the units' ranges sit at the end of the scratch
  * block's partial accumulators, which the plan then uses less of. */
 static int ts_run_mod(fa_problem *p, void *scratch, void *stream) {
+    if (ts_few_rows(p)) {
+        ts_scratch s;
+        ts_scratch_layout(scratch, p->D, &s);
+        p->status = s.status;
+        p->part_m = s.m;
+        p->part_l = s.l;
+        p->part_acc = s.acc;
+        return ts_launch_few_rows(p, stream);
+    }
     if (p->mod && (p->key_begin || p->key_end) && p->Sq > TS_MOD_INLINE_ROWS && ts_tc_supported(p)) {
         ts_scratch s;
         ts_scratch_layout(scratch, p->D, &s);

@@ -82,6 +82,10 @@ int ts_launch_attention(const fa_problem *p, void *stream);
  * tensor-core launch with modified scores. */
 int ts_launch_mod_bounds(const fa_problem *p, void *stream);
 int ts_launch_tc_mod(const fa_problem *p, void *stream);
+/* Modified scores for few query rows of each kv head (fa_rows.cu): whether a problem is one, and its
+ * launch (status and part_* set). */
+int ts_few_rows(const fa_problem *p);
+int ts_launch_few_rows(const fa_problem *p, void *stream);
 /* Key ranges of packed documents (fa_mod.cu), see attn_mask_ranges_stream. */
 int ts_launch_mask_ranges(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,
                           int *key_begin, int *key_end, void *stream);

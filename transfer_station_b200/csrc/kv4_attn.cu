@@ -39,14 +39,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-
 #include "attn_kv4.h"
 #include "fa_launch.h"
+#include "rows_plan.cuh"
 #include "score_cap.cuh"
-#include "sm100_ptx.cuh"
-
-extern "C" void ts_count_launch(void);
 
 namespace ts {
 
@@ -56,26 +52,12 @@ constexpr int kTile = 128;       // keys per stage
 constexpr int kWarps = 4;        // consumer warps, 32 keys of a tile each
 constexpr int kSlabs = 2;        // 16-key MMA rows of a warp and tile
 constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kMinTiles = 1;     // a CTA takes at least this many tiles (fewer CTAs work on small problems)
 
 constexpr float kHead = 4.f, kMost = 7.f;  // see the weights
 
-struct Kv4Params {
-    const uint16_t *Q;
+struct Kv4Params : RowsParams {
     const uint8_t *kc, *ks, *vc, *vs;
-    const int *block_table, *seq_lens;
-    void *O;
-    int o_bf16;
-    int B, Hq, Hkv, Sq, group, row_blocks, causal;
-    int page_size, num_pages, max_pages;
-    float scale_log2;  // log2(e) / sqrt(D)
     float cap_in, cap_out, tanh_k[5];
-    const float *slopes;
-    const int *key_begin, *key_end;
-    int *status;                  // [0]: result; [2], [3]: reports of the running call and its generation
-    unsigned gen;
-    float *part_m, *part_l, *part_acc;  // [2 * CTAs][rows]([D]): slot 2c of CTA c for a unit begun before it, 2c + 1 after
-    int2 *desc;                   // [units]: first and last CTA of a unit (equal: nothing to merge)
 };
 
 template <int D, int NT>
@@ -106,12 +88,6 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-    uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
-
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
 
@@ -119,20 +95,6 @@ __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast
 __device__ __forceinline__ __half2 scales2(uint32_t bytes) {
     const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)bytes, __NV_E4M3);
     return __half2(r);
-}
-
-// Four 8x8 matrices of 16-bit elements; lane l gives the address of row l % 8 of matrix l / 8.
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // fp16: n * 2^-24, n * 2^-20
@@ -146,133 +108,6 @@ __device__ __forceinline__ uint32_t centre_low(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t centre_high(uint32_t x) {
     return as_u32(__hfma2(as_half2(x & kHigh), as_half2(kTwo11), as_half2(kMinusEight)));
-}
-
-// A sequence: its keys, the span [lo, hi) outside which no query of it sees one, and the tiles of that
-// span (at least one, so that a sequence without keys gets its zero rows). The span is read from the key
-// ranges for up to kSpanRows query positions; longer calls walk the whole sequence.
-constexpr int kSpanRows = 16;
-struct Span {
-    int len, lo, hi, t0, nt;
-};
-__device__ __forceinline__ Span seq_span(const Kv4Params &p, int b) {
-    Span s;
-    const int n = ld_plan(p.seq_lens + b), most = p.max_pages * p.page_size;
-    s.len = n < 0 ? 0 : (n < most ? n : most);
-    s.lo = 0;
-    s.hi = s.len;
-    if ((p.key_begin || p.key_end) && p.Sq <= kSpanRows) {
-        int lo = s.len, hi = 0;
-        for (int i = 0; i < p.Sq; ++i) {
-            const size_t at = (size_t)b * p.Sq + i;
-            lo = min(lo, p.key_begin ? ld_plan(p.key_begin + at) : 0);
-            hi = max(hi, p.key_end ? ld_plan(p.key_end + at) : s.len);
-        }
-        s.lo = max(lo, 0);
-        s.hi = min(hi, s.len);
-    }
-    s.t0 = s.lo / kTile;
-    s.nt = s.hi > s.lo ? (s.hi + kTile - 1) / kTile - s.t0 : 1;
-    return s;
-}
-
-// Where a CTA's share of the tile list begins, and what the list is.
-struct Share {
-    long long total, t0, t1;  // all tiles; this CTA's
-    int ctas;                 // CTAs that have a share
-    int b;                    // first sequence
-    int u;                    // first unit within it
-    int tile;                 // first tile of that unit's span
-};
-
-// All threads of the CTA. Units are ordered by sequence, then kv head, then row block.
-__device__ __forceinline__ Share find_share(const Kv4Params &p, int cta, int grid) {
-    __shared__ long long warp_sum[32];
-    __shared__ long long found_rem;
-    __shared__ int found_b;
-    const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = n >> 5;
-    const int units = p.Hkv * p.row_blocks;
-    const int chunk = (p.B + n - 1) / n;
-    const int b0 = min(p.B, tid * chunk), b1 = min(p.B, b0 + chunk);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (long long)seq_span(p, b).nt * units;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) warp_sum[warp] = incl;
-    if (tid == 0) found_b = p.B;
-    __syncthreads();
-    long long before = 0, total = 0;
-    for (int w = 0; w < warps; ++w) {
-        if (w < warp) before += warp_sum[w];
-        total += warp_sum[w];
-    }
-    Share s;
-    s.total = total;
-    const long long most = (total + kMinTiles - 1) / kMinTiles;
-    s.ctas = (int)(most < grid ? most : grid);
-    s.t0 = cta < s.ctas ? cta * total / s.ctas : total;
-    s.t1 = cta < s.ctas ? (cta + 1) * total / s.ctas : total;
-    long long at = before + incl - mine;
-    if (s.t0 >= at && s.t0 < at + mine) {
-        int b = b0;
-        for (; b < b1; ++b) {
-            const long long here = (long long)seq_span(p, b).nt * units;
-            if (s.t0 < at + here) break;
-            at += here;
-        }
-        found_b = b;
-        found_rem = s.t0 - at;
-    }
-    __syncthreads();
-    s.b = found_b;
-    s.u = s.tile = 0;
-    if (s.t0 < s.t1) {
-        const int nt = seq_span(p, s.b).nt;
-        s.u = (int)(found_rem / nt);
-        s.tile = (int)(found_rem - (long long)s.u * nt);
-    }
-    return s;
-}
-
-// The CTA that has tile x of the list.
-__device__ __forceinline__ int owner(long long x, long long total, int ctas) {
-    int c = (int)(x * ctas / total);
-    while (c + 1 < ctas && (c + 1) * total / ctas <= x) ++c;
-    return c;
-}
-
-// Reports gather in a pair (generation, codes) that kv4_combine moves to the status word: a report can
-// neither meet the clearing of an earlier call's nor be lost by a replayed graph's.
-__device__ __forceinline__ void report_pending(const Kv4Params &p, int code) {
-    unsigned long long *at = reinterpret_cast<unsigned long long *>(p.status + 2);
-    unsigned long long old = *reinterpret_cast<volatile unsigned long long *>(at);
-    while (true) {
-        const unsigned long long now = (unsigned)(old >> 32) == p.gen ? old | (unsigned)code
-                                                                      : ((unsigned long long)p.gen << 32) | (unsigned)code;
-        const unsigned long long seen = atomicCAS(at, old, now);
-        if (seen == old) return;
-        old = seen;
-    }
-}
-
-// Bounded wait on a barrier of this CTA.
-__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, const Kv4Params &p,
-                                          int code) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (true) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            *abort_flag = 1;
-            report_pending(p, code);
-            return false;
-        }
-    }
 }
 
 // A slab's 16 rows of codes: lane (g, t) gets word t of every group of rows g and g + 8, or transposed the
@@ -322,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     }
     pdl_wait();
     pdl_trigger();
-    const Share sh = find_share(p, blockIdx.x, gridDim.x);  // (its barriers also publish the set-up)
+    const Share sh = find_share<kTile>(p, blockIdx.x, gridDim.x);  // (its barriers also publish the set-up)
     if (sh.t0 >= sh.t1) return;
 
     const int units = p.Hkv * p.row_blocks;
@@ -338,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         uint32_t round = 0;
         bool ok = true;
         while (left > 0 && ok) {
-            const Span sp = seq_span(p, b);
+            const Span sp = seq_span<kTile>(p, b);
             const int len = sp.len, nt = sp.nt;
             const int kvh = u / p.row_blocks;
             const int used = (len + P - 1) / P;
@@ -424,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     uint32_t phase = 0;
     bool ok = true;
     while (left > 0) {
-        const Span span = seq_span(p, b);
+        const Span span = seq_span<kTile>(p, b);
         const int len = span.len, nt = span.nt;
         const int kvh = u / p.row_blocks, rb = u - kvh * p.row_blocks;
         const int begin = tile, end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
@@ -794,87 +629,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     }
 }
 
-// Merges a cut unit's partials: block (unit, row), its warps take pieces in turn. Block 0 also moves the
-// call's reports to the status word.
-template <int D, int NT>
-__global__ void __launch_bounds__(128) kv4_combine(const Kv4Params p) {
-    constexpr int ROWS = 8 * NT, PER = D / 32;
-    __shared__ float sm[4], sl[4], sacc[4][D];
-    pdl_wait();
-    pdl_trigger();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-        unsigned long long *at = reinterpret_cast<unsigned long long *>(p.status + 2);
-        const unsigned long long v = *reinterpret_cast<volatile unsigned long long *>(at);
-        p.status[0] = (unsigned)(v >> 32) == p.gen ? (int)(unsigned)v : 0;
-        *at = 0;
-    }
-    const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.Hkv * p.row_blocks;
-    const int2 d = make_int2(ld_plan(&p.desc[blockIdx.x].x), ld_plan(&p.desc[blockIdx.x].y));
-    if (d.x == d.y) return;
-    const int b = blockIdx.x / units, u = blockIdx.x - b * units;
-    const int kvh = u / p.row_blocks, rb = u - kvh * p.row_blocks;
-    const int row = rb * ROWS + r, rows_all = p.group * p.Sq;
-    if (row >= rows_all) return;
-    auto slot = [&](int c) { return ((size_t)2 * c + (c == d.x ? 1 : 0)) * ROWS + r; };
-    float m = -INFINITY, l = 0.f, acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    for (int c = d.x + warp; c <= d.y; c += 4) {
-        const size_t at = slot(c);
-        const float mc = p.part_m[at], lc = p.part_l[at];
-        float v[PER];
-        if constexpr (PER == 4) {
-            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p.part_acc + at * D + PER * lane);
-        } else {
-            *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p.part_acc + at * D + PER * lane);
-        }
-        const float to = fmaxf(m, mc);
-        const float f0 = m == -INFINITY ? 0.f : ex2(m - to), f1 = mc == -INFINITY ? 0.f : ex2(mc - to);
-        l = l * f0 + lc * f1;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = acc[i] * f0 + v[i] * f1;
-        m = to;
-    }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sacc[warp][PER * lane + i] = acc[i];
-    __syncthreads();
-    const int col = threadIdx.x;
-    if (col >= D) return;
-    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float L = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - M);
-        L = fmaf(f, sl[w], L);
-        o = fmaf(f, sacc[w][col], o);
-    }
-    const float inv = L > 0.f ? 1.f / (kUnit * L) : (L == 0.f ? 0.f : L);
-    const size_t at = (((size_t)b * p.Hkv + kvh) * rows_all + row) * D + col;
-    if (p.o_bf16)
-        reinterpret_cast<uint16_t *>(p.O)[at] = (uint16_t)pack_bf16x2(o * inv, 0.f);
-    else
-        reinterpret_cast<float *>(p.O)[at] = o * inv;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // A code pool as {D/2 bytes, rows of a page, page x kv head}, boxes of one page's rows up to a tile.
 bool make_code_map(CUtensorMap *m, const uint8_t *codes, const ts_kv4_problem *P, int D) {
-    static const EncodeTiledFn fn = []() -> EncodeTiledFn {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            return reinterpret_cast<EncodeTiledFn>(ptr);
-        return nullptr;
-    }();
+    const EncodeTiledFn fn = encode_tiled();
     if (!fn) return false;
     const cuuint64_t row = (cuuint64_t)D / 2, ps = (cuuint64_t)P->page_size;
     cuuint64_t dims[3] = {row, ps, (cuuint64_t)P->num_pages * P->Hkv};
@@ -886,84 +643,39 @@ bool make_code_map(CUtensorMap *m, const uint8_t *codes, const ts_kv4_problem *P
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename... KArgs, typename... Args>
-int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return ATTN_ERR_CUDA;
-    ts_count_launch();
-    return ATTN_OK;
-}
-
-// CTAs of this kernel that fit on an SM (cached per device, with the shared-memory opt-in done).
-template <int D, int NT, bool MOD>
-int resident() {
-    static std::atomic<int> cache[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return -1;
-    const bool cached = dev >= 0 && dev < 64;
-    if (cached) {
-        const int r = cache[dev].load(std::memory_order_acquire);
-        if (r > 0) return r;
-    }
-    auto kern = kv4_kernel<D, NT, MOD>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv4Config<D, NT>::SMEM) != cudaSuccess)
-        return -1;
-    int r = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r, kern, kThreads, Kv4Config<D, NT>::SMEM) != cudaSuccess || r < 1)
-        r = 1;
-    if (cached) cache[dev].store(r, std::memory_order_release);
-    return r;
-}
-
 template <int D, int NT, bool MOD>
 int run(const ts_kv4_problem *P, cudaStream_t st) {
-    const int fit = resident<D, NT, MOD>();
+    static std::atomic<int> cache[64];
+    const int fit = resident(kv4_kernel<D, NT, MOD>, kThreads, Kv4Config<D, NT>::SMEM, cache);
     if (fit < 0) return ATTN_ERR_CUDA;
     Kv4Params p;
     p.Q = P->Q;
-    p.kc = P->k_codes, p.ks = P->k_scales, p.vc = P->v_codes, p.vs = P->v_scales;
-    p.block_table = P->block_table;
-    p.seq_lens = P->seq_lens;
     p.O = P->O;
     p.o_bf16 = P->o_bf16;
-    p.B = P->B, p.Hq = P->Hq, p.Hkv = P->Hkv, p.Sq = P->Sq;
+    p.B = P->B, p.Hkv = P->Hkv, p.Sq = P->Sq, p.D = D;
     p.group = P->Hq / P->Hkv;
-    p.row_blocks = (p.group * P->Sq + 8 * NT - 1) / (8 * NT);
     p.causal = P->causal;
+    p.block_table = P->block_table;
+    p.seq_lens = P->seq_lens;
     p.page_size = P->page_size, p.num_pages = P->num_pages, p.max_pages = P->max_pages;
+    p.Sk = P->max_pages * P->page_size;
     p.scale_log2 = P->scale_log2;
-    p.cap_in = P->cap_in, p.cap_out = P->cap_out;
-    for (int i = 0; i < 5; ++i) p.tanh_k[i] = P->cap_out * kTanhC[i];
     p.slopes = P->slopes;
     p.key_begin = P->key_begin, p.key_end = P->key_end;
     p.status = P->status;
-    p.gen = ts_next_status_gen();
-    const long long units = (long long)P->B * P->Hkv * p.row_blocks;
-    const long long tiles = ((long long)P->max_pages * P->page_size + kTile - 1) / kTile;
-    long long ctas = (long long)ts_num_sms() * fit;
-    if (ctas > P->part_rows / (2 * 8 * NT)) ctas = P->part_rows / (2 * 8 * NT);
-    if (tiles * units < ctas) ctas = tiles * units;
-    // the partials: rows of the first 2 * ctas slots; the units' descriptors behind their accumulators
-    p.part_m = P->part_m;
-    p.part_l = P->part_l;
-    p.part_acc = P->part_acc;
-    const size_t acc = (size_t)2 * ctas * 8 * NT * D;
-    if (acc * 4 + (size_t)units * sizeof(int2) > (size_t)P->part_rows * D * 4) return ATTN_ERR_ARGS;
-    p.desc = reinterpret_cast<int2 *>(P->part_acc + acc);
+    p.unit = kUnit;
+    p.part_m = P->part_m, p.part_l = P->part_l, p.part_acc = P->part_acc;
+    p.kc = P->k_codes, p.ks = P->k_scales, p.vc = P->v_codes, p.vs = P->v_scales;
+    p.cap_in = P->cap_in, p.cap_out = P->cap_out;
+    for (int i = 0; i < 5; ++i) p.tanh_k[i] = P->cap_out * kTanhC[i];
+    int ctas = 0;
+    const int planned = plan_rows<kTile, D, 8 * NT>(p, fit, P->part_rows, ctas);
+    if (planned != ATTN_OK) return planned;
     CUtensorMap tmK, tmV;
     if (!make_code_map(&tmK, P->k_codes, P, D) || !make_code_map(&tmV, P->v_codes, P, D)) return ATTN_ERR_CUDA;
     const int rc = launch(kv4_kernel<D, NT, MOD>, dim3((unsigned)ctas), dim3(kThreads), Kv4Config<D, NT>::SMEM, st, tmK, tmV, p);
     if (rc != ATTN_OK) return rc;
-    return launch(kv4_combine<D, NT>, dim3((unsigned)units, 8 * NT), dim3(128), 0, st, p);
+    return launch_combine<D, 8 * NT>(p, st);
 }
 
 }  // namespace
