@@ -8,8 +8,12 @@
 // about 200 other instructions for 16 keys, while their 8 KB take it 1,400 cycles to arrive.
 //
 // One producer warp streams 64-key tiles by TMA (128-byte swizzle, the layout ldmatrix reads without bank
-// conflicts) into a 192 KB ring; four consumer warps take 16 keys of each, with a running maximum and an
-// accumulator of their own, merged in shared memory at a unit's end. The work split is rows_plan.cuh's.
+// conflicts) into a 96 KB ring; four consumer warps take 16 keys of each, with a running maximum and an
+// accumulator of their own, merged in shared memory at a unit's end. Two such CTAs share an SM, so that one
+// streams while the other is between units (one CTA with twice the ring: 64 sequences of 300 keys 39 us, not
+// 31). The work split is rows_plan.cuh's.
+//
+// Measured, 16 sequences of 8,192 keys, 4 rows, D = 128, cap: 52.8 us of 42.3 for the bytes (ragged lengths).
 #include <cuda_bf16.h>
 
 #include <atomic>
@@ -38,14 +42,16 @@ struct FewConfig {
     static constexpr int HALF = kTile * 128;           // 64 elements of a tile's keys
     static constexpr int TILE_BYTES = HALF * (DP / 64);
     static constexpr int STAGE = 2 * TILE_BYTES;       // K, V
-    static constexpr int NS = 196608 / STAGE;
+    static constexpr int NS = 98304 / STAGE;
     static constexpr int ROWS = 8 * NT;
-    static constexpr int MERGE = kWarps * ROWS * (DP + 4) * 4;
+    static constexpr int ROUNDS = NT * DP / 64;        // of the merge, to fit two CTAs on an SM
+    static constexpr int COLS = DP / ROUNDS;
+    static constexpr int MERGE = kWarps * ROWS * (COLS + 4) * 4;
     static constexpr int OFF_MERGE = NS * STAGE;
     static constexpr int OFF_ML = OFF_MERGE + MERGE;   // m, l [kWarps][ROWS]
     static constexpr int OFF_BAR = OFF_ML + 2 * kWarps * ROWS * 4;
     static constexpr int SMEM = OFF_BAR + 2 * NS * 8 + 1024;  // + alignment of the swizzled tiles
-    static_assert(SMEM <= 227 * 1024, "");
+    static_assert(2 * (SMEM + 2048) <= 228 * 1024, "");
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -55,7 +61,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 template <int DP, int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const FewParams p) {
     using C = FewConfig<DP, NT>;
     constexpr int KT = DP / 16;  // 16-element steps of the first product, tiles of the output
@@ -382,14 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ml[warp * C::ROWS + 8 * n + 2 * t + c] = most[n][c] == -INFINITY ? -INFINITY : ref[n][c];
                     ml[(kWarps + warp) * C::ROWS + 8 * n + 2 * t + c] = l[n][c];
                 }
-                float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (DP + 4) + g;
-#pragma unroll
-                for (int k = 0; k < KT; ++k) {
-                    dst[16 * k] = acc[n][k][c];
-                    dst[16 * k + 8] = acc[n][k][c + 2];
-                }
             }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
         const bool cut = begin > 0 || end < nt;
         const size_t slot = ((size_t)2 * blockIdx.x + (begin > 0 ? 0 : 1)) * C::ROWS;
         if (threadIdx.x == 0 && begin == 0) {
@@ -400,41 +399,57 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             p.desc[(size_t)b * units + u] = d;
         }
-        constexpr int V4 = DP / 4;
-        for (int x = threadIdx.x; x < C::ROWS * V4; x += 32 * kWarps) {
-            const int r = x / V4, c4 = x - r * V4;
-            float mw[kWarps], M = -INFINITY, L = 0.f;
+        constexpr int V4 = C::COLS / 4;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                mw[w] = ml[w * C::ROWS + r];
-                M = fmaxf(M, mw[w]);
-            }
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int round = 0; round < C::ROUNDS; ++round) {
+            const int col0 = round * C::COLS;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
-                const float4 v = *reinterpret_cast<const float4 *>(merge + (w * C::ROWS + r) * (DP + 4) + 4 * c4);
-                L = fmaf(f, ml[(kWarps + w) * C::ROWS + r], L);
-                o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-            }
-            if (cut) {
-                if (c4 == 0) {
-                    p.part_m[slot + r] = M;
-                    p.part_l[slot + r] = L;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float *dst = merge + (warp * C::ROWS + 8 * n + 2 * t + c) * (C::COLS + 4) + g;
+#pragma unroll
+                    for (int k = 0; k < C::COLS / 16; ++k) {
+                        dst[16 * k] = acc[n][round * (C::COLS / 16) + k][c];
+                        dst[16 * k + 8] = acc[n][round * (C::COLS / 16) + k][c + 2];
+                    }
                 }
-                *reinterpret_cast<float4 *>(p.part_acc + (slot + r) * DP + 4 * c4) = o;
-            } else if (row0 + r < rows_all && 4 * c4 < D) {
-                const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-                const size_t at = (qrow0 + r) * D + 4 * c4;
-                if (p.o_bf16)
-                    *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.O) + at) =
-                        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                else
-                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.O) + at) =
-                        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+            for (int x = threadIdx.x; x < C::ROWS * V4; x += 32 * kWarps) {
+                const int r = x / V4, c4 = x - r * V4, col = col0 + 4 * c4;
+                float mw[kWarps], M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    mw[w] = ml[w * C::ROWS + r];
+                    M = fmaxf(M, mw[w]);
+                }
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
+                    const float4 v = *reinterpret_cast<const float4 *>(merge + (w * C::ROWS + r) * (C::COLS + 4) + 4 * c4);
+                    L = fmaf(f, ml[(kWarps + w) * C::ROWS + r], L);
+                    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+                }
+                if (cut) {
+                    if (col == 0) {
+                        p.part_m[slot + r] = M;
+                        p.part_l[slot + r] = L;
+                    }
+                    *reinterpret_cast<float4 *>(p.part_acc + (slot + r) * DP + col) = o;
+                } else if (row0 + r < rows_all && col < D) {
+                    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+                    const size_t at = (qrow0 + r) * D + col;
+                    if (p.o_bf16)
+                        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.O) + at) =
+                            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                    else
+                        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.O) + at) =
+                            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                }
             }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");  // the merge area is free again
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");  // the merge area is free again
         left -= end - begin;
         tile = 0;
         if (++u == units) {
@@ -496,7 +511,9 @@ int run(const fa_problem *P, cudaStream_t st) {
 }  // namespace ts
 
 extern "C" int ts_few_rows(const fa_problem *P) {
-    // (as many units as descriptors find room behind the partials; key indexes look a few tiles past the end)
+    // More than 16 rows would read the cache twice, from L2: 16 sequences of 8,192 keys, capped, took here and
+    // in the kernel for prompts 117 and 164 us at 16 rows, 195 and 166 at 24 (one of 32,768: 47 and 55, 64 and 57).
+    // (As many units as descriptors find room behind the partials; key indexes look a few tiles past the end.)
     return P->mod && (long long)(P->Hq / P->Hkv) * P->Sq <= 16 && P->Hkv <= 65536 && P->Sk <= 0x7fffffff - 65536 &&
            ts_tc_supported(P);
 }

@@ -327,7 +327,8 @@ int plan_rows(RowsParams &p, int fit, int part_rows, int &ctas) {
 
 template <int D, int ROWS>
 int launch_combine(const RowsParams &p, cudaStream_t st) {
-    return launch(rows_combine<D, ROWS>, dim3((unsigned)((long long)p.B * p.Hkv * p.row_blocks), ROWS), dim3(128), 0, st, p);
+    const int rows = p.group * p.Sq < ROWS ? p.group * p.Sq : ROWS;
+    return launch(rows_combine<D, ROWS>, dim3((unsigned)((long long)p.B * p.Hkv * p.row_blocks), rows), dim3(128), 0, st, p);
 }
 
 }  // namespace
