@@ -148,6 +148,7 @@ static void ts_plan_core(fa_problem *p, int tc, int sms, int ctas) {
 static void ts_plan(fa_problem *p) {
     const int tc = ts_tc_supported(p);
     const long long rows = (long long)p->Hq * p->Sq;
+    if (p->order) return; /* whole units (ts_fill's plan), sorted by their lengths */
     ts_plan_core(p, tc, ts_num_sms(), tc ? ts_tc_ctas_per_split(p) : (int)((rows + 7) / 8));
 }
 
@@ -319,8 +320,8 @@ static int ts_set_mod(fa_problem *p, const attn_mod *mod, int Hkv) {
  * from a kernel of their own first (about 2 us, against 256 dependent reads per unit and role). */
 #define TS_MOD_INLINE_ROWS 8
 
-/* Runs a problem with modified scores. The bounds of the units' ranges sit at the end of the scratch
- * block's partial accumulators, which the plan then uses less of. */
+/* Runs a problem with modified scores. The bounds of the units' ranges and the units' order sit at the end
+ * of the scratch block's partial accumulators, which the plan then uses less of. */
 static int ts_run_mod(fa_problem *p, void *scratch, void *stream) {
     if (ts_few_rows(p)) {
         ts_scratch s;
@@ -331,16 +332,23 @@ static int ts_run_mod(fa_problem *p, void *scratch, void *stream) {
         p->part_acc = s.acc;
         return ts_launch_few_rows(p, stream);
     }
-    if (p->mod && (p->key_begin || p->key_end) && p->Sq > TS_MOD_INLINE_ROWS && ts_tc_supported(p)) {
-        ts_scratch s;
-        ts_scratch_layout(scratch, p->D, &s);
-        const size_t units = (size_t)(p->Hkv / p->hkv_local) * (size_t)(ts_tc_ctas_per_split(p) / p->Hkv);
+    if (p->mod && ts_tc_supported(p)) {
+        const int ranges = p->key_begin || p->key_end, per_kv = ts_tc_ctas_per_split(p) / p->Hkv;
+        const long long units = (long long)per_kv * p->Hkv, tiles = units / p->hkv_local;
+        /* units of different lengths that the kernel's own order would not put longest first */
+        const int misfit = p->causal && p->Hq != p->Hkv && p->Sq % ts_tc_unit_rows(p) != 0;
+        const int order = units > ts_num_sms() && (ranges || p->paged || misfit);
         const size_t row_bytes = (size_t)p->D * sizeof(float);
-        const size_t taken = (units * 4 * sizeof(int) + row_bytes - 1) / row_bytes + 1;
-        if (taken <= ATTN_PARTIAL_ROWS / 2) { /* else: the kernel reads the ranges itself */
+        const size_t bytes = (size_t)tiles * 8 * sizeof(int) + (order ? (size_t)units * sizeof(int) : 0);
+        const size_t taken = (bytes + row_bytes - 1) / row_bytes + 1;
+        /* no room: the kernel reads the ranges itself */
+        if ((order || (ranges && p->Sq > TS_MOD_INLINE_ROWS)) && taken <= ATTN_PARTIAL_ROWS / 2) {
+            ts_scratch s;
+            ts_scratch_layout(scratch, p->D, &s);
             p->part_cap = ATTN_PARTIAL_ROWS - (int)taken;
-            /* 16-byte aligned, within the rows taken (one more than the bounds fill) */
+            /* 16-byte aligned, within the rows taken (one more than they fill) */
             p->bounds = (int *)(((uintptr_t)(s.acc + (size_t)p->part_cap * (size_t)p->D) + 15u) & ~(uintptr_t)15u);
+            if (order) p->order = p->bounds + 8 * tiles;
         }
     }
     return ts_run(p, scratch, stream);

@@ -93,10 +93,13 @@ struct TcParams {
     unsigned gen;
     // Modified scores (MOD != 0 only). A query position's keys are [key_begin, key_end) (device
     // arrays [B][Sq], either may be null) within the causal limit; the kv index is
-    // b * hkv_local + kv_local. bounds (when not null): [B][tiles_per_kv], over a unit's rows the least
-    // begin and greatest end of those that see a key, the greatest begin and least end of all.
+    // b * hkv_local + kv_local. bounds (when not null): [B][tiles_per_kv][2], over a unit's rows the least
+    // begin and greatest end of those that see a key, the greatest begin and least end of all; then a range
+    // between that no row sees (a unit may hold the end of one query head and the start of the next).
+    // order (when not null): the units, the longest first.
     const int *key_begin, *key_end;
     const int4 *bounds;
+    const int *order;
     const float *slopes;  // [query heads of one sequence]: distance bias
     float cap_in;         // 1 / (cap * sqrt(D)): raw score -> argument of tanh
     float cap_out;        // cap * log2(e)
@@ -227,12 +230,14 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         int ulo, uhi;      // MOD: no row of the unit sees a key outside [ulo, uhi) ...
         int ilo, ihi;      // ... and every row sees every key of [ilo, ihi)
         int near;          // MOD with a distance bias: the block the walk begins with
+        int hole, skip;    // MOD: from the hole-th block on, skip blocks that no row sees are passed over
     };
     // The item's j-th key block. With a distance bias the walk begins at the unit's own position and goes
     // back, then ahead: weights fall on the way, where walking from the far end would raise every row's
     // maximum at every block.
     auto block_of = [&](const Item &it, int j) {
-        if constexpr (MOD >= kModBias) return j <= it.near ? it.near - j : j;
+        if constexpr (MOD >= kModBias) j = j <= it.near ? it.near - j : j;
+        if constexpr (MOD != 0) j += j < it.hole ? 0 : it.skip;
         return j;
     };
     auto item_at = [&](int q) {
@@ -254,7 +259,9 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             }
         } else {
             int u = q;
-            if (MOD != 0 && p.causal && p.pieces == 1) {  // whole units, the longest first (as below)
+            if (MOD != 0 && p.order) {
+                u = ld_plan(p.order + q);
+            } else if (MOD != 0 && p.causal && p.pieces == 1) {  // whole units, the longest first (as below)
                 const int hk = p.Hkv * p.group;
                 if (p.head_units > 0) {
                     const int rem = q % hk;
@@ -289,12 +296,16 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         if constexpr (MOD != 0) {
             it.ulo = it.ilo = 0;
             it.uhi = it.ihi = it.sk;
+            it.hole = it.skip = 0;
             if (p.bounds) {
-                const int4 w = ld_plan(p.bounds + (size_t)(it.kv / p.hkv_local) * p.tiles_per_kv + tile);
+                const int4 *at = p.bounds + 2 * ((size_t)(it.kv / p.hkv_local) * p.tiles_per_kv + tile);
+                const int4 w = ld_plan(at), h = ld_plan(at + 1);
                 it.ulo = max(0, w.x);
                 it.uhi = min(it.uhi, w.y);
                 it.ilo = max(0, w.z);
                 it.ihi = min(it.ihi, w.w);
+                it.hole = h.x;  // (keys, for now)
+                it.skip = h.y;
             } else if (p.key_begin || p.key_end) {  // few query positions: read them all
                 const size_t at = (size_t)(it.kv / p.hkv_local) * p.Sq;
                 int lo = 0x7fffffff, hi = 0, lo1 = 0, hi1 = it.sk;
@@ -325,9 +336,17 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             if (it.ulo > it.kb0) it.kb0 += (it.ulo - it.kb0) / kBN * kBN;
         }
         it.nblk = kend > it.kb0 ? (kend - it.kb0 + kBN - 1) / kBN : 0;
+        if constexpr (MOD != 0) {
+            const int h0 = max(it.hole - it.kb0 + kBN - 1, 0) / kBN, h1 = min(max(it.skip - it.kb0, 0) / kBN, it.nblk);
+            it.hole = h0;
+            it.skip = max(h1 - h0, 0);
+            it.nblk -= it.skip;
+        }
         if constexpr (MOD >= kModBias) {
             const int pos = it.sk_total - p.Sq + it.row0 % p.Sq;
-            it.near = p.causal ? it.nblk - 1 : max(0, min((pos - it.kb0) / kBN, it.nblk - 1));
+            int at = max(pos - it.kb0, 0) / kBN;
+            if (at >= it.hole) at = max(it.hole, at - it.skip);
+            it.near = p.causal ? it.nblk - 1 : max(0, min(at, it.nblk - 1));
         }
         return it;
     };
@@ -1450,6 +1469,7 @@ static int launch_tc(const fa_problem *P, cudaStream_t st, int tiles_per_kv) {
     prm.key_begin = P->key_begin;
     prm.key_end = P->key_end;
     prm.bounds = reinterpret_cast<const int4 *>(P->bounds);
+    prm.order = P->order;
     prm.slopes = P->slopes;
     prm.cap_in = P->cap_in;
     prm.cap_out = P->cap_out;
@@ -1468,7 +1488,7 @@ static int launch_tc(const fa_problem *P, cudaStream_t st, int tiles_per_kv) {
     }
     if constexpr (MOD != 0) {
         prm.n_items = prm.n_direct + (units - prm.n_direct) * prm.pieces;
-        prm.snake = prm.causal && prm.pieces == 1;
+        prm.snake = (prm.causal && prm.pieces == 1) || prm.order;
         if (P->paged)
             return launch_tc_inst<DP, NQT, false, true, true, false, MOD>(st, tmQ, tmK, tmV, tmO, prm,
                                                                           dim3(min(prm.n_items, sms)));

@@ -53,11 +53,12 @@ typedef struct fa_problem {
     unsigned status_gen;
     /* Modified scores (attn_flash_mod_stream; mod 0: none): 1 key ranges only, 2 cap, 3 distance
      * bias, 4 both. Key ranges [B][Sq] (either may be NULL) apply with every mod; kv head index =
-     * b * hkv_local + kv_local. bounds: scratch room for the per-unit range bounds, or NULL (the
-     * kernel then reads a unit's ranges itself). */
+     * b * hkv_local + kv_local. bounds: scratch room for the per-unit range bounds (8 ints a sequence
+     * and row tile), or NULL (the kernel then reads a unit's ranges itself). order: room for the units
+     * in the order of their lengths (with bounds, one piece a unit), or NULL. */
     int mod;
     const int *key_begin, *key_end;
-    int *bounds;
+    int *bounds, *order;
     const float *slopes;       /* [Hq of one sequence] */
     float cap_in, cap_out;     /* 1 / (cap * sqrt(D)), cap * log2(e) */
     int part_cap;              /* partial rows the plan may use (0: ATTN_PARTIAL_ROWS) */
@@ -78,7 +79,7 @@ int ts_tc_unit_rows(const fa_problem *p);
  * !write_partials, the combine kernel. Returns 0 or a negative ATTN_ERR_* code. */
 int ts_launch_attention(const fa_problem *p, void *stream);
 
-/* Fill p->bounds (one int pair per sequence and row tile of a kv head) from the key ranges, and the
+/* Fill p->bounds from the key ranges, the causal rule and the lengths, and p->order from those; and the
  * tensor-core launch with modified scores. */
 int ts_launch_mod_bounds(const fa_problem *p, void *stream);
 int ts_launch_tc_mod(const fa_problem *p, void *stream);

@@ -15,62 +15,126 @@ extern "C" int ts_launch_tc_mod4(const fa_problem *P, void *stream);
 
 namespace ts {
 
+constexpr int kBlock = ATTN_GPU_KEY_TILE;  // keys of the attention kernel's block
+constexpr int kBins = 2048;
+
 // One warp per (sequence, row tile of a kv head): the least begin and greatest end over the tile's
-// query positions that see a key ({0, 0} when none does), the greatest begin and least end of all. Rows of a tile are packed (query head,
-// position), so positions repeat; a tile of at least Sq rows covers all of them.
-__global__ void __launch_bounds__(256) mod_bounds_kernel(const int *__restrict__ key_begin,
-                                                         const int *__restrict__ key_end, int4 *__restrict__ out,
-                                                         int n, int tiles, int unit_rows, int rows_per_kv, int Sq, int Sk) {
+// query positions that see a key ({0, 0} when none does), the greatest begin and least end of all. Rows of a
+// tile are packed (query head, position), so positions repeat; a tile of at least Sq rows covers all of them.
+// A tile across the border of two query heads holds the last positions and the first: between what the two
+// parts see may lie a hole, {begin, end} of the second int4, whose third member is the tile's key blocks.
+__global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
+                                                         const int *key_end,
+                                                         const int *seq_lens, int4 *out,
+                                                         int n, int tiles, int unit_rows, int rows_per_kv, int Sq, int Smax,
+                                                         int causal) {
     pdl_wait();
     pdl_trigger();
     const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (w >= n) return;
     const int b = w / tiles, row0 = (w - b * tiles) * unit_rows;
-    const int rows = min(min(unit_rows, rows_per_kv - row0), Sq);
+    const int rows = min(min(unit_rows, rows_per_kv - row0), Sq), i0 = row0 % Sq;
+    const int Sk = seq_lens ? max(0, min(ld_plan(seq_lens + b), Smax)) : Smax;
     const size_t at = (size_t)b * Sq;
-    int lo = 0x7fffffff, hi = 0, lo1 = 0, hi1 = Sk;
+    int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0}, lo1 = 0, hi1 = Sk;  // [1]: past the border
     for (int e = lane; e < rows; e += 32) {
-        const int i = (row0 + e) % Sq;
-        const int b0 = key_begin ? key_begin[at + i] : 0, b1 = key_end ? key_end[at + i] : Sk;
+        const int past = i0 + e >= Sq, i = i0 + e - (past ? Sq : 0);
+        const int b0 = key_begin ? max(ld_plan(key_begin + at + i), 0) : 0;
+        int b1 = key_end ? min(ld_plan(key_end + at + i), Sk) : Sk;
+        if (causal) b1 = min(b1, Sk - Sq + i + 1);
         if (b0 < b1) {
-            lo = min(lo, b0);
-            hi = max(hi, b1);
+            lo[past] = min(lo[past], b0);
+            hi[past] = max(hi[past], b1);
         }
         lo1 = max(lo1, b0);
         hi1 = min(hi1, b1);
     }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        lo[h] = __reduce_min_sync(0xffffffffu, lo[h]);
+        hi[h] = __reduce_max_sync(0xffffffffu, hi[h]);
+    }
     lo1 = __reduce_max_sync(0xffffffffu, lo1);
     hi1 = __reduce_min_sync(0xffffffffu, hi1);
-    if (lane == 0) out[w] = hi > lo ? make_int4(lo, hi, lo1, hi1) : make_int4(0, 0, 0, 0);
+    if (lane != 0) return;
+    const int a = min(lo[0], lo[1]), z = max(hi[0], hi[1]);
+    if (z <= a) {
+        out[2 * w] = out[2 * w + 1] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    int h0 = 0, h1 = 0;
+    if (hi[0] > 0 && hi[1] > 0) {
+        const int first = lo[1] < lo[0];  // the part whose keys come first
+        if (hi[first] < lo[1 - first]) h0 = hi[first], h1 = lo[1 - first];
+    }
+    // blocks from the first key's on, less whole ones of the hole (as the attention kernel walks them)
+    const int base = a / kBlock * kBlock, skip = h1 > h0 ? (h1 - base) / kBlock - (h0 - base + kBlock - 1) / kBlock : 0;
+    out[2 * w] = make_int4(a, z, lo1, hi1);
+    out[2 * w + 1] = make_int4(h0, h1, (z - base + kBlock - 1) / kBlock - max(skip, 0), 0);
+}
+
+// The units, longest first: a counting sort of the tiles by their key blocks (in steps of 2^shift blocks),
+// every tile standing for its sequence's kv heads. The order of equal ones is arbitrary; no result depends
+// on it.
+__global__ void __launch_bounds__(1024) mod_order_kernel(const int4 *bounds, int *order, int n,
+                                                         int tiles, int hkv, int shift) {
+    __shared__ int count[kBins], warp_sum[32];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < kBins; i += 1024) count[i] = 0;
+    __syncthreads();
+    // bin 0: the longest
+    auto bin = [&](int w) { return kBins - 1 - min(ld_plan(bounds + 2 * w + 1).z >> shift, kBins - 1); };
+    for (int w = tid; w < n; w += 1024) atomicAdd(&count[bin(w)], hkv);
+    __syncthreads();
+    // exclusive sums: two bins a thread
+    static_assert(kBins == 2048, "");
+    const int c0 = count[2 * tid], c1 = count[2 * tid + 1];
+    int incl = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int before = incl - c0 - c1;
+    for (int i = 0; i < warp; ++i) before += warp_sum[i];
+    count[2 * tid] = before;
+    count[2 * tid + 1] = before + c0;
+    __syncthreads();
+    for (int w = tid; w < n; w += 1024) {
+        const int at = atomicAdd(&count[bin(w)], hkv), b = w / tiles, tile = w - b * tiles;
+        for (int h = 0; h < hkv; ++h) order[at + h] = (b * hkv + h) * tiles + tile;
+    }
 }
 
 // Token i of document [s, e) sees keys [s, i] and the document's first prefix tokens (causal), or the
 // whole document; with a window only its last `window` keys. The document is found by bisection.
-__global__ void __launch_bounds__(256) mask_ranges_kernel(const int *__restrict__ cu, const int *__restrict__ prefix,
+__global__ void __launch_bounds__(256) mask_ranges_kernel(const int *cu, const int *prefix,
                                                           int n_docs, int S, int causal, int window,
-                                                          int *__restrict__ key_begin, int *__restrict__ key_end) {
+                                                          int *key_begin, int *key_end) {
     pdl_wait();
     pdl_trigger();
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= S) return;
     int begin = 0, end = 0;
-    if (i >= cu[0] && i < cu[n_docs]) {
+    if (i >= ld_plan(cu) && i < ld_plan(cu + n_docs)) {
         int a = 0, b = n_docs;  // cu[a] <= i < cu[b]
         while (b - a > 1) {
             const int m = (a + b) >> 1;
-            if (cu[m] <= i)
+            if (ld_plan(cu + m) <= i)
                 a = m;
             else
                 b = m;
         }
-        const int s = cu[a], e = min(cu[a + 1], S);
+        const int s = ld_plan(cu + a), e = min(ld_plan(cu + a + 1), S);
         begin = s;
         end = e;
         if (causal) {
             end = i + 1;
-            if (prefix) end = max(end, (int)min((long long)e, (long long)s + prefix[a]));
+            if (prefix) end = max(end, (int)min((long long)e, (long long)s + ld_plan(prefix + a)));
         }
         if (window > 0) begin = max(begin, i - window + 1);
     }
@@ -79,10 +143,10 @@ __global__ void __launch_bounds__(256) mask_ranges_kernel(const int *__restrict_
 }
 
 template <typename... KArgs, typename... Args>
-static int launch(void (*kern)(KArgs...), unsigned grid, cudaStream_t st, Args... args) {
+static int launch(void (*kern)(KArgs...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(block);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -98,14 +162,20 @@ static int launch(void (*kern)(KArgs...), unsigned grid, cudaStream_t st, Args..
 
 extern "C" int ts_launch_mod_bounds(const fa_problem *P, void *stream) {
     const int tiles = ts_tc_ctas_per_split(P) / P->Hkv, n = P->Hkv / P->hkv_local * tiles;
-    return ts::launch(ts::mod_bounds_kernel, (unsigned)((n + 7) / 8), static_cast<cudaStream_t>(stream), P->key_begin,
-                      P->key_end, reinterpret_cast<int4 *>(P->bounds), n, tiles, ts_tc_unit_rows(P),
-                      P->Hq / P->Hkv * P->Sq, P->Sq, P->Sk);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int4 *bounds = reinterpret_cast<int4 *>(P->bounds);
+    const int rc = ts::launch(ts::mod_bounds_kernel, (unsigned)((n + 7) / 8), 256, st, P->key_begin, P->key_end,
+                              P->paged ? P->seq_lens : nullptr, bounds, n, tiles, ts_tc_unit_rows(P),
+                              P->Hq / P->Hkv * P->Sq, P->Sq, P->Sk, P->causal);
+    if (rc != ATTN_OK || !P->order) return rc;
+    int shift = 0;
+    while (((P->Sk - 1) / ts::kBlock + 1) >> shift >= ts::kBins) ++shift;
+    return ts::launch(ts::mod_order_kernel, 1u, 1024, st, bounds, P->order, n, tiles, P->hkv_local, shift);
 }
 
 extern "C" int ts_launch_mask_ranges(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,
                                      int *key_begin, int *key_end, void *stream) {
-    return ts::launch(ts::mask_ranges_kernel, (unsigned)(((long long)S + 255) / 256), static_cast<cudaStream_t>(stream), cu_docs,
+    return ts::launch(ts::mask_ranges_kernel, (unsigned)(((long long)S + 255) / 256), 256, static_cast<cudaStream_t>(stream), cu_docs,
                       prefix, n_docs, S, causal, window, key_begin, key_end);
 }
 
