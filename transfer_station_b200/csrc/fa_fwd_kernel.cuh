@@ -95,7 +95,8 @@ struct TcParams {
     // arrays [B][Sq], either may be null) within the causal limit; the kv index is
     // b * hkv_local + kv_local. bounds (when not null): [B][tiles_per_kv][2], over a unit's rows the least
     // begin and greatest end of those that see a key, the greatest begin and least end of all; then a range
-    // between that no row sees (a unit may hold the end of one query head and the start of the next).
+    // between that no row sees (a unit may hold the end of one query head and the start of the next), the
+    // key blocks, and whether some row sees each key from the least begin to the greatest end.
     // order (when not null): the units, the longest first.
     const int *key_begin, *key_end;
     const int4 *bounds;
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         int sk, sk_total;  // keys present (local) and the key axis length the causal rule uses
         int ulo, uhi;      // MOD: no row of the unit sees a key outside [ulo, uhi) ...
         int ilo, ihi;      // ... and every row sees every key of [ilo, ihi)
+        bool solid;        // some row sees each key of [ulo, uhi)
         int near;          // MOD with a distance bias: the block the walk begins with
         int hole, skip;    // MOD: from the hole-th block on, skip blocks that no row sees are passed over
     };
@@ -297,6 +299,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             it.ulo = it.ilo = 0;
             it.uhi = it.ihi = it.sk;
             it.hole = it.skip = 0;
+            it.solid = !p.key_begin && !p.key_end;
             if (p.bounds) {
                 const int4 *at = p.bounds + 2 * ((size_t)(it.kv / p.hkv_local) * p.tiles_per_kv + tile);
                 const int4 w = ld_plan(at), h = ld_plan(at + 1);
@@ -306,6 +309,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 it.ihi = min(it.ihi, w.w);
                 it.hole = h.x;  // (keys, for now)
                 it.skip = h.y;
+                it.solid = h.w != 0;
             } else if (p.key_begin || p.key_end) {  // few query positions: read them all
                 const size_t at = (size_t)(it.kv / p.hkv_local) * p.Sq;
                 int lo = 0x7fffffff, hi = 0, lo1 = 0, hi1 = it.sk;
@@ -1132,9 +1136,9 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             // V rows that no row of the unit sees (what an unused slot holds, a key between two
             // ranges) become zero before P V reads them: 0 * NaN would reach every row. PV_0 is
             // issued first, after every thread of this warpgroup arrived.
-            if (t == 0 && (key0 < it.ilo || key0 + kBN > it.ihi)) {
+            if (t == 0 && (it.solid ? key0 < it.ulo || key0 + kBN > it.uhi : key0 < it.ilo || key0 + kBN > it.ihi)) {
                 bool keep = key0 + r >= it.ulo && key0 + r < it.uhi;
-                if (p.key_begin || p.key_end) {
+                if (!it.solid) {
                     // the union of both tiles' rows as 128 bits, a word per 32 keys
                     uint32_t *buf = seen_bits + 16 * (seen_turn & 1);
                     ++seen_turn;

@@ -22,7 +22,9 @@ constexpr int kBins = 2048;
 // query positions that see a key ({0, 0} when none does), the greatest begin and least end of all. Rows of a
 // tile are packed (query head, position), so positions repeat; a tile of at least Sq rows covers all of them.
 // A tile across the border of two query heads holds the last positions and the first: between what the two
-// parts see may lie a hole, {begin, end} of the second int4, whose third member is the tile's key blocks.
+// parts see may lie a hole, {begin, end} of the second int4, whose third member is the tile's key blocks and
+// whose fourth says that some row sees each key from the least begin to the greatest end: within a part
+// the rows that see keys follow one another, and each one's range touches the next one's.
 __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
                                                          const int *key_end,
                                                          const int *seq_lens, int4 *out,
@@ -37,14 +39,24 @@ __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
     const int Sk = seq_lens ? max(0, min(ld_plan(seq_lens + b), Smax)) : Smax;
     const size_t at = (size_t)b * Sq;
     int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0}, lo1 = 0, hi1 = Sk;  // [1]: past the border
+    int runs[2] = {0, 0}, apart = 0;  // runs of rows that see keys, neighbours that do not touch
+    auto keys = [&](int i, int &b0, int &b1) {
+        b0 = key_begin ? max(ld_plan(key_begin + at + i), 0) : 0;
+        b1 = key_end ? min(ld_plan(key_end + at + i), Sk) : Sk;
+        if (causal) b1 = min(b1, Sk - Sq + i + 1);
+    };
     for (int e = lane; e < rows; e += 32) {
         const int past = i0 + e >= Sq, i = i0 + e - (past ? Sq : 0);
-        const int b0 = key_begin ? max(ld_plan(key_begin + at + i), 0) : 0;
-        int b1 = key_end ? min(ld_plan(key_end + at + i), Sk) : Sk;
-        if (causal) b1 = min(b1, Sk - Sq + i + 1);
+        int b0, b1, c0 = 0, c1 = 0;
+        keys(i, b0, b1);
+        if (e > 0 && i > 0) keys(i - 1, c0, c1);  // the row before
         if (b0 < b1) {
             lo[past] = min(lo[past], b0);
             hi[past] = max(hi[past], b1);
+            if (c0 >= c1)
+                ++runs[past];
+            else
+                apart |= max(b0, c0) > min(b1, c1);
         }
         lo1 = max(lo1, b0);
         hi1 = min(hi1, b1);
@@ -53,7 +65,9 @@ __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
     for (int h = 0; h < 2; ++h) {
         lo[h] = __reduce_min_sync(0xffffffffu, lo[h]);
         hi[h] = __reduce_max_sync(0xffffffffu, hi[h]);
+        runs[h] = __reduce_add_sync(0xffffffffu, runs[h]);
     }
+    apart = __any_sync(0xffffffffu, apart);
     lo1 = __reduce_max_sync(0xffffffffu, lo1);
     hi1 = __reduce_min_sync(0xffffffffu, hi1);
     if (lane != 0) return;
@@ -70,7 +84,8 @@ __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
     // blocks from the first key's on, less whole ones of the hole (as the attention kernel walks them)
     const int base = a / kBlock * kBlock, skip = h1 > h0 ? (h1 - base) / kBlock - (h0 - base + kBlock - 1) / kBlock : 0;
     out[2 * w] = make_int4(a, z, lo1, hi1);
-    out[2 * w + 1] = make_int4(h0, h1, (z - base + kBlock - 1) / kBlock - max(skip, 0), 0);
+    out[2 * w + 1] = make_int4(h0, h1, (z - base + kBlock - 1) / kBlock - max(skip, 0),
+                             runs[0] <= 1 && runs[1] <= 1 && !apart && h1 <= h0);
 }
 
 // The units, longest first: a counting sort of the tiles by their key blocks (in steps of 2^shift blocks),
