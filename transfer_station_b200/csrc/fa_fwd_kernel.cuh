@@ -1047,6 +1047,31 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 }
                 tmem_st8(tS + (c0 >> 1), pk);
             };
+            // The running maximum for a block whose maximum is mb, and what its scores are taken less; then, with
+            // the block's row sums in acc0 and acc1, the sum and the accumulator under the new maximum.
+            float m_new, alpha;
+            auto raise = [&](float mb) {
+                m_new = m;
+                if (mb > m && (m == -INFINITY || mb - m > kRescaleLog2)) m_new = mb;
+                alpha = (m_new == m) ? 1.f : ((m == -INFINITY) ? 0.f : ex2(m - m_new));
+                return (m_new == -INFINITY) ? 0.f : m_new;
+            };
+            auto settle = [&]() {
+                l = l * alpha + ((acc0.x + acc1.x) + (acc0.y + acc1.y));
+                m = m_new;
+                // O_t holds P V through the block before (complete: these scores were committed after it).
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                    for (int cc = 0; cc < DP / 32; ++cc) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + cc * 32, o);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[u] = f2u(u2f(o[u]) * alpha);
+                        tmem_st32(tO + cc * 32, o);
+                    }
+                }
+            };
+            constexpr bool kRangeOnly = MOD == kModRange;
             bool general = !none && !fixed;
             if (none) {
                 uint32_t zero[16];
@@ -1061,8 +1086,63 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     weigh(c0, x);
                 });
                 l += (acc0.x + acc1.x) + (acc0.y + acc1.y);
+            } else if (kRangeOnly) {
+                // The scores stay in registers, in two unrolled passes (masks, maximum; exponentials) when the
+                // speculation is not taken or fails: a block that some row sees in part takes 2 us less than by
+                // the rolled loops below, which read the score tile twice.
+                uint32_t sr[128];
+                if (spec) {
+                    const float2 m2 = make_float2(-m, -m);
+                    tmem_ld16p(tS, sr);
+#pragma unroll
+                    for (int cc = 0; cc < 8; ++cc) {
+                        float2 x[8];
+                        if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            x[u] = __ffma2_rn(make_float2(u2f(sr[16 * cc + 2 * u]), u2f(sr[16 * cc + 2 * u + 1])), c2, m2);
+                        weigh(16 * cc, x);
+                        if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
+                    }
+                    const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
+                    general = __any_sync(0xffffffffu, rs > kRedoSum);
+                    if (!general) l += rs;
+                    acc0 = acc1 = make_float2(0.f, 0.f);
+                } else {
+#pragma unroll
+                    for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + 32 * cc, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * cc));
+                }
+                if (general) {
+                    if (!full) {
+#pragma unroll
+                        for (int cc = 0; cc < 4; ++cc) {
+                            const uint32_t w = span_bits(n0 - 32 * cc, n1 - 32 * cc);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u)
+                                if (!((w >> u) & 1u)) sr[32 * cc + u] = 0xff800000u;
+                        }
+                    }
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < 64; u += 2) {
+                        mx0 = fmax3(mx0, u2f(sr[2 * u]), u2f(sr[2 * u + 1]));
+                        mx1 = fmax3(mx1, u2f(sr[2 * u + 2]), u2f(sr[2 * u + 3]));
+                    }
+                    const float ref = raise(__fmul_rn(fmaxf(mx0, mx1), p.scale_log2));
+                    const float2 ref2 = make_float2(-ref, -ref);
+#pragma unroll
+                    for (int cc = 0; cc < 8; ++cc) {
+                        float2 x[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            x[u] = __ffma2_rn(make_float2(u2f(sr[16 * cc + 2 * u]), u2f(sr[16 * cc + 2 * u + 1])), c2, ref2);
+                        weigh(16 * cc, x);
+                    }
+                    settle();
+                    general = false;
+                }
             } else if (spec) {
-                if constexpr (!kCap) {
+                if constexpr (!kCap && !kRangeOnly) {
                     uint32_t sr[128];
                     const float t0 = b0 - m;
                     const float2 bs2 = make_float2(bs, bs), t02 = make_float2(t0, t0);
@@ -1107,11 +1187,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                             mx0 = fmax3(mx0, z[u].x, z[u].y);
                     }
                 });
-                const float mb = fmaxf(mx0, mx1);
-                float m_new = m;
-                if (mb > m && (m == -INFINITY || mb - m > kRescaleLog2)) m_new = mb;
-                const float alpha = (m_new == m) ? 1.f : ((m == -INFINITY) ? 0.f : ex2(m - m_new));
-                const float ref = (m_new == -INFINITY) ? 0.f : m_new;
+                const float ref = raise(fmaxf(mx0, mx1));
                 chunks([&](int c0, const uint32_t *raw) {
                     float2 z[8];
                     scores(std::false_type{}, raw, c0, 0.f, z);  // then the subtraction: a row's largest weighs exactly 1
@@ -1119,19 +1195,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     for (int u = 0; u < 8; ++u) z[u] = __fadd2_rn(z[u], make_float2(-ref, -ref));
                     weigh(c0, z);
                 });
-                l = l * alpha + ((acc0.x + acc1.x) + (acc0.y + acc1.y));
-                m = m_new;
-                // O_t holds P V through the block before (complete: these scores were committed after it).
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-                    for (int cc = 0; cc < DP / 32; ++cc) {
-                        uint32_t o[32];
-                        tmem_ld32(tO + cc * 32, o);
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) o[u] = f2u(u2f(o[u]) * alpha);
-                        tmem_st32(tO + cc * 32, o);
-                    }
-                }
+                settle();
             }
             // V rows that no row of the unit sees (what an unused slot holds, a key between two
             // ranges) become zero before P V reads them: 0 * NaN would reach every row. PV_0 is
