@@ -949,9 +949,10 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             // The choice must be warp-uniform: every path issues warp-collective tcgen05.st.
             const bool full = __all_sync(0xffffffffu, n0 == 0 && n1 == kBN);
             const bool none = __all_sync(0xffffffffu, n1 <= n0);
-            // a distance bias is linear in the key on each side of the query position
-            const bool past = !kBias || __all_sync(0xffffffffu, key0 + kBN - 1 <= qpos);
-            const bool ahead = kBias && __all_sync(0xffffffffu, key0 >= qpos);
+            // a distance bias is linear in the key on each side of the query position: over all keys that the warp's
+            // rows see, or not
+            const bool past = !kBias || __all_sync(0xffffffffu, key0 + n1 - 1 <= qpos);
+            const bool ahead = kBias && __all_sync(0xffffffffu, key0 + n0 >= qpos);
             const float bs = past ? slope2 : -slope2;
             const float b0 = kBias ? bs * (float)(key0 - (past ? qpos - near : qpos + near)) : 0.f;
             const bool fixed = kCap && p.cap_ref >= 0.f;
@@ -1071,7 +1072,6 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     }
                 }
             };
-            constexpr bool kRangeOnly = MOD == kModRange;
             bool general = !none && !fixed;
             if (none) {
                 uint32_t zero[16];
@@ -1086,91 +1086,77 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     weigh(c0, x);
                 });
                 l += (acc0.x + acc1.x) + (acc0.y + acc1.y);
-            } else if (kRangeOnly) {
-                // The scores stay in registers, in two unrolled passes (masks, maximum; exponentials) when the
-                // speculation is not taken or fails: a block that some row sees in part takes 2 us less than by
-                // the rolled loops below, which read the score tile twice.
-                uint32_t sr[128];
-                if (spec) {
-                    const float2 m2 = make_float2(-m, -m);
-                    tmem_ld16p(tS, sr);
-#pragma unroll
-                    for (int cc = 0; cc < 8; ++cc) {
-                        float2 x[8];
-                        if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            x[u] = __ffma2_rn(make_float2(u2f(sr[16 * cc + 2 * u]), u2f(sr[16 * cc + 2 * u + 1])), c2, m2);
-                        weigh(16 * cc, x);
-                        if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
-                    }
-                    const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
-                    general = __any_sync(0xffffffffu, rs > kRedoSum);
-                    if (!general) l += rs;
-                    acc0 = acc1 = make_float2(0.f, 0.f);
-                } else {
-#pragma unroll
-                    for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + 32 * cc, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * cc));
-                }
-                if (general) {
-                    if (!full) {
-#pragma unroll
-                        for (int cc = 0; cc < 4; ++cc) {
-                            const uint32_t w = span_bits(n0 - 32 * cc, n1 - 32 * cc);
-#pragma unroll
-                            for (int u = 0; u < 32; ++u)
-                                if (!((w >> u) & 1u)) sr[32 * cc + u] = 0xff800000u;
-                        }
-                    }
-                    float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < 64; u += 2) {
-                        mx0 = fmax3(mx0, u2f(sr[2 * u]), u2f(sr[2 * u + 1]));
-                        mx1 = fmax3(mx1, u2f(sr[2 * u + 2]), u2f(sr[2 * u + 3]));
-                    }
-                    const float ref = raise(__fmul_rn(fmaxf(mx0, mx1), p.scale_log2));
-                    const float2 ref2 = make_float2(-ref, -ref);
-#pragma unroll
-                    for (int cc = 0; cc < 8; ++cc) {
-                        float2 x[8];
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            x[u] = __ffma2_rn(make_float2(u2f(sr[16 * cc + 2 * u]), u2f(sr[16 * cc + 2 * u + 1])), c2, ref2);
-                        weigh(16 * cc, x);
-                    }
-                    settle();
-                    general = false;
-                }
-            } else if (spec) {
-                if constexpr (!kCap && !kRangeOnly) {
+            } else if (!kCap && (past || ahead)) {
+                // The scores stay in registers, in two unrolled passes (bias, masks, maximum; exponentials) when
+                // the speculation is not taken or fails: a block that some row sees in part takes 2 us less
+                // than by the rolled loops below, which read the score tile twice.
+                if constexpr (!kCap) {
                     uint32_t sr[128];
-                    const float t0 = b0 - m;
-                    const float2 bs2 = make_float2(bs, bs), t02 = make_float2(t0, t0);
-                    tmem_ld16p(tS, sr);
+                    const float2 bs2 = make_float2(bs, bs);
+                    auto linear = [&](int c, float2 add) {  // scores of columns c, c + 1, and the bias
+                        return __ffma2_rn(make_float2(u2f(sr[c]), u2f(sr[c + 1])), c2,
+                                          kBias ? __ffma2_rn(make_float2((float)c, (float)(c + 1)), bs2, add) : add);
+                    };
+                    if (spec) {
+                        const float2 less = make_float2(b0 - m, b0 - m);
+                        tmem_ld16p(tS, sr);
 #pragma unroll
-                    for (int cc = 0; cc < 8; ++cc) {
-                        float2 x[8];
-                        if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
+                        for (int cc = 0; cc < 8; ++cc) {
+                            float2 x[8];
+                            if (cc < 7) tmem_ld16_nowait(tS + 16 * (cc + 1), sr + 16 * (cc + 1));
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int c = 16 * cc + 2 * u;
-                            const float2 at = kBias ? __ffma2_rn(make_float2((float)c, (float)(c + 1)), bs2, t02) : t02;
-                            x[u] = __ffma2_rn(make_float2(u2f(sr[c]), u2f(sr[c + 1])), c2, at);
+                            for (int u = 0; u < 8; ++u) x[u] = linear(16 * cc + 2 * u, less);
+                            weigh(16 * cc, x);
+                            if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
                         }
-                        weigh(16 * cc, x);
-                        if (cc < 7) tmem_wait_ld16(sr + 16 * (cc + 1));
-                    }
-                    const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
-                    general = __any_sync(0xffffffffu, rs > kRedoSum);
-                    if (!general) {
-                        l += rs;
-                    } else {  // the raw scores go back under the P stored over them
-                        tmem_wait_st();
+                        const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
+                        general = __any_sync(0xffffffffu, rs > kRedoSum);
+                        if (!general) l += rs;
+                        acc0 = acc1 = make_float2(0.f, 0.f);
+                    } else {
 #pragma unroll
                         for (int cc = 0; cc < 4; ++cc)
-                            tmem_st32(tS + 32 * cc, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * cc));
-                        tmem_wait_st();
-                        acc0 = acc1 = make_float2(0.f, 0.f);
+                            tmem_ld32(tS + 32 * cc, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * cc));
+                    }
+                    if (general) {
+                        if (kBias) {
+                            const float2 add = make_float2(b0, b0);
+#pragma unroll
+                            for (int u = 0; u < 64; ++u) {
+                                const float2 z = linear(2 * u, add);
+                                sr[2 * u] = f2u(z.x), sr[2 * u + 1] = f2u(z.y);
+                            }
+                        }
+                        if (!full) {
+#pragma unroll
+                            for (int cc = 0; cc < 4; ++cc) {
+                                const uint32_t w = span_bits(n0 - 32 * cc, n1 - 32 * cc);
+#pragma unroll
+                                for (int u = 0; u < 32; ++u)
+                                    if (!((w >> u) & 1u)) sr[32 * cc + u] = 0xff800000u;
+                            }
+                        }
+                        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < 64; u += 2) {
+                            mx0 = fmax3(mx0, u2f(sr[2 * u]), u2f(sr[2 * u + 1]));
+                            mx1 = fmax3(mx1, u2f(sr[2 * u + 2]), u2f(sr[2 * u + 3]));
+                        }
+                        const float mb = fmaxf(mx0, mx1), ref = raise(kBias ? mb : __fmul_rn(mb, p.scale_log2));
+                        const float2 less = make_float2(-ref, -ref);
+#pragma unroll
+                        for (int cc = 0; cc < 8; ++cc) {
+                            float2 x[8];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) {
+                                const int c = 16 * cc + 2 * u;
+                                const float2 z = make_float2(u2f(sr[c]), u2f(sr[c + 1]));
+                                x[u] = kBias ? __fadd2_rn(z, less) : __ffma2_rn(z, c2, less);
+                            }
+                            weigh(16 * cc, x);
+                        }
+                        settle();
+                        general = false;
                     }
                 }
             }
