@@ -12,6 +12,7 @@ anything itself -- if the library is missing it raises, there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 from typing import NamedTuple
@@ -171,11 +172,21 @@ def _ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 
 
+@functools.cache
+def _current_stream():
+    """A function that returns the current stream's handle. torch.cuda.current_stream() makes a Stream object,
+    3.3 us of a 13 us call; where torch has it, the handle alone (0.3 us) is asked for."""
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None:
+        return lambda: torch.cuda.current_stream().cuda_stream
+    return lambda: raw(torch.cuda.current_device())
+
+
 def _stream_handle(stream) -> int:
     if stream is None:
-        import torch
-
-        return int(torch.cuda.current_stream().cuda_stream)
+        return int(_current_stream()())
     return int(getattr(stream, "cuda_stream", stream))
 
 
