@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     float *ml = reinterpret_cast<float *>(smem + C::OFF_ML);
     const int rows_all = p.group * p.Sq, D = p.D;
     const bool has_cap = p.cap_out > 0.f, has_bias = p.slopes != nullptr;
+    const float fac1 = has_cap ? p.cap_in : p.scale_log2, fac[2] = {fac1, fac1};
     // ldmatrix: matrix m = lane / 8 is keys 8 (m % 2) .. of chunk m / 2 for K (an A operand), keys 8 (m / 2) ..
     // of chunk m % 2 for V (transposed to one); a chunk: 16 bytes, swizzled by the key's low bits.
     const int r8 = lane & 7, m8 = lane >> 3;
@@ -204,8 +205,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                     qf[n][i][h] = have && 16 * i + 8 * h < D ? *reinterpret_cast<const uint32_t *>(src + 16 * i + 8 * h) : 0u;
         }
         // ---- this lane's query columns: keys seen, position, bias
-        int lo[NT][2], hi[NT][2], pos[NT][2], near[NT][2];
-        float slope2[NT][2];
+        int lo[NT][2], hi[NT][2], pos[NT][2];
+        float slope2[NT][2], near[NT][2];
         int all_lo = 0, all_hi = len;  // every row sees [all_lo, all_hi)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (p.key_begin) lo[n][c] = min(max(0, ld_plan(p.key_begin + at)), len);
                 if (p.key_end) hi[n][c] = min(hi[n][c], ld_plan(p.key_end + at));
                 hi[n][c] = max(hi[n][c], 0);
-                near[n][c] = max(0, max(lo[n][c] - pos[n][c], pos[n][c] - (hi[n][c] - 1)));
+                near[n][c] = (float)max(0, max(lo[n][c] - pos[n][c], pos[n][c] - (hi[n][c] - 1)));
                 slope2[n][c] = has_bias ? ld_plan(p.slopes + kvh * p.group + row / p.Sq) * 1.4426950408889634f : 0.f;
                 all_lo = max(all_lo, lo[n][c]);
                 all_hi = min(all_hi, hi[n][c]);
@@ -271,22 +272,29 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int c = e & 1;
-                        const float raw = s[n][e] + s1[n][e];
-                        float z;
-                        if (has_cap) {
-                            const float y = raw * p.cap_in, w = y * y;
-                            z = cap_far(y, y * tanh_poly(make_float2(w, w), p.tanh_k).x, p.cap_out) - ref[n][c];
-                        } else {
-                            z = fmaf(raw, p.scale_log2, -ref[n][c]);
-                        }
-                        if (has_bias) {
-                            const int key = key0 + g + 8 * (e >> 1);
-                            z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
-                        }
-                        s[n][e] = z;
+                    for (int e = 0; e < 4; ++e) s[n][e] += s1[n][e];
+                if (has_cap) {
+                    float far = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) cap_argument(s[n], fac, far);
+                    if (__any_sync(0xffffffffu, far > kTanhMaxSq)) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) cap_any(s[n], p.tanh_k, p.cap_out, ref[n]);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) cap_near(s[n], p.tanh_k, ref[n]);
                     }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) scale_less(s[n], fac, ref[n]);
+                }
+                if (has_bias) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float at[2] = {(float)(key0 - pos[n][0] + g), (float)(key0 - pos[n][1] + g)};
+                        less_bias(s[n], 0.f, at, near[n], slope2[n]);
+                    }
+                }
                 const bool whole = key0 >= all_lo && key0 + 16 <= all_hi;
                 uint32_t v_keep[2] = {0xffffffffu, 0xffffffffu};  // keys 2t, 2t + 1 and 2t + 8, 2t + 9
                 if (!whole) {

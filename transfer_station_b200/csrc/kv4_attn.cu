@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
             fac[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * unit;
         }
         // ---- this lane's query columns: keys seen, position, bias
-        int lo[NT][2], hi[NT][2], pos[NT][2], near[NT][2];
-        float slope2[NT][2];
+        int lo[NT][2], hi[NT][2], pos[NT][2];
+        float slope2[NT][2], near[NT][2];
         int all_lo = 0, all_hi = len;  // every row sees [all_lo, all_hi)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                 if (p.key_begin) lo[n][c] = min(max(0, ld_plan(p.key_begin + at)), len);
                 if (p.key_end) hi[n][c] = min(hi[n][c], ld_plan(p.key_end + at));
                 hi[n][c] = max(hi[n][c], 0);
-                near[n][c] = max(0, max(lo[n][c] - pos[n][c], pos[n][c] - (hi[n][c] - 1)));
+                near[n][c] = (float)max(0, max(lo[n][c] - pos[n][c], pos[n][c] - (hi[n][c] - 1)));
                 slope2[n][c] = has_bias ? ld_plan(p.slopes + kvh * p.group + row / p.Sq) * 1.4426950408889634f : 0.f;
                 all_lo = max(all_lo, lo[n][c]);
                 all_hi = min(all_hi, hi[n][c]);
@@ -412,26 +412,37 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                 // ---- scores less their column's reference, log2 units: element e is key g + 8 (e / 2) of its
                 // slab, query column e % 2
                 const bool whole = key0 >= all_lo && key0 + 16 * kSlabs <= all_hi;
+                if (has_cap) {
+                    float far = 0.f;
 #pragma unroll
-                for (int b = 0; b < kSlabs; ++b)
+                    for (int b = 0; b < kSlabs; ++b)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                        for (int n = 0; n < NT; ++n) cap_argument(s[b][n], fac[n], far);
+                    if (__any_sync(0xffffffffu, far > kTanhMaxSq)) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int c = e & 1;
-                            float z;
-                            if (has_cap) {
-                                const float y = s[b][n][e] * fac[n][c], w = y * y;
-                                z = cap_far(y, y * tanh_poly(make_float2(w, w), p.tanh_k).x, p.cap_out) - ref[n][c];
-                            } else {
-                                z = fmaf(s[b][n][e], fac[n][c], -ref[n][c]);
-                            }
-                            if (has_bias) {
-                                const int key = key0 + 16 * b + g + 8 * (e >> 1);
-                                z = fmaf(-slope2[n][c], fabsf((float)(key - pos[n][c])) - (float)near[n][c], z);
-                            }
-                            s[b][n][e] = z;
-                        }
+                        for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) cap_any(s[b][n], p.tanh_k, p.cap_out, ref[n]);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) cap_near(s[b][n], p.tanh_k, ref[n]);
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) scale_less(s[b][n], fac[n], ref[n]);
+                }
+                if (has_bias) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float at[2] = {(float)(key0 - pos[n][0] + g), (float)(key0 - pos[n][1] + g)};
+#pragma unroll
+                        for (int b = 0; b < kSlabs; ++b) less_bias(s[b][n], 16.f * b, at, near[n], slope2[n]);
+                    }
+                }
                 if (!whole) {
 #pragma unroll
                     for (int b = 0; b < kSlabs; ++b)

@@ -29,4 +29,45 @@ __device__ __forceinline__ float cap_far(float y, float inside, float cap_out, f
     return y * y > kTanhMaxSq ? outer : inside;
 }
 
+// The scores of kernels with keys as the matrix rows, a lane's four at a time: keys g and g + 8 (elements 0, 1 and
+// 2, 3), two query columns (elements 0, 2 and 1, 3), each column with its factor, reference, position.
+__device__ __forceinline__ void cap_argument(float (&s)[4], const float (&fac)[2], float &far) {  // -> y, the largest y^2
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+        const float2 y = __fmul2_rn(make_float2(s[h], s[h + 1]), make_float2(fac[0], fac[1]));
+        s[h] = y.x, s[h + 1] = y.y;
+        far = fmax3(far, y.x * y.x, y.y * y.y);
+    }
+}
+__device__ __forceinline__ void cap_near(float (&s)[4], const float (&k)[5], const float (&ref)[2]) {
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+        const float2 y = make_float2(s[h], s[h + 1]);
+        const float2 z = __ffma2_rn(y, tanh_poly(__fmul2_rn(y, y), k), make_float2(-ref[0], -ref[1]));
+        s[h] = z.x, s[h + 1] = z.y;
+    }
+}
+__device__ __forceinline__ void cap_any(float (&s)[4], const float (&k)[5], float cap_out, const float (&ref)[2]) {
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+        const float2 y = make_float2(s[h], s[h + 1]), z = __fmul2_rn(y, tanh_poly(__fmul2_rn(y, y), k));
+        s[h] = cap_far(y.x, z.x, cap_out) - ref[0];
+        s[h + 1] = cap_far(y.y, z.y, cap_out) - ref[1];
+    }
+}
+__device__ __forceinline__ void scale_less(float (&s)[4], const float (&fac)[2], const float (&ref)[2]) {
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+        const float2 z = __ffma2_rn(make_float2(s[h], s[h + 1]), make_float2(fac[0], fac[1]), make_float2(-ref[0], -ref[1]));
+        s[h] = z.x, s[h + 1] = z.y;
+    }
+}
+// at: key g less the column's position; off: further keys on (exact sums: a context of 2^24 keys is past every use)
+__device__ __forceinline__ void less_bias(float (&s)[4], float off, const float (&at)[2], const float (&near)[2],
+                                          const float (&slope2)[2]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        s[e] = fmaf(-slope2[e & 1], fabsf(at[e & 1] + (off + 4.f * (e & 2))) - near[e & 1], s[e]);
+}
+
 }  // namespace ts
