@@ -106,6 +106,7 @@ def test_paged_rows(cuda_dev, P, D):
     (1, 24, 2, 1601, 1777, 64, 1, 30.0, 0, 1),
     (3, 16, 8, 900, 1000, 128, 1, 30.0, 1, 1),
     (5, 20, 20, 300, 640, 128, 0, 0.0, 1, 1),
+    (1100, 1, 1, 20, 90, 64, 0, 0.0, 0, 1),       # more sequences than are ranked one against all
 ])
 def test_sorted_units(cuda_dev, B, Hq, Hkv, Sq, Sk, D, causal, cap, bias, ranged):
     run(B, Hq, Hkv, Sq, Sk, D, causal, cap, bias, ranged, torch.bfloat16, cuda_dev, Sq)

@@ -17,6 +17,7 @@ namespace ts {
 
 constexpr int kBlock = ATTN_GPU_KEY_TILE;  // keys of the attention kernel's block
 constexpr int kBins = 2048;
+constexpr int kMostRows = 256;             // of a unit
 
 // One warp per (sequence, row tile of a kv head): the least begin and greatest end over the tile's
 // query positions that see a key ({0, 0} when none does), the greatest begin and least end of all. Rows of a
@@ -25,41 +26,54 @@ constexpr int kBins = 2048;
 // parts see may lie a hole, {begin, end} of the second int4, whose third member is the tile's key blocks and
 // whose fourth says that some row sees each key from the least begin to the greatest end: within a part
 // the rows that see keys follow one another, and each one's range touches the next one's.
-__global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
-                                                         const int *key_end,
-                                                         const int *seq_lens, int4 *out,
-                                                         int n, int tiles, int unit_rows, int rows_per_kv, int Sq, int Smax,
-                                                         int causal) {
-    pdl_wait();
-    pdl_trigger();
-    const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (w >= n) return;
-    const int b = w / tiles, row0 = (w - b * tiles) * unit_rows;
-    const int rows = min(min(unit_rows, rows_per_kv - row0), Sq), i0 = row0 % Sq;
-    const int Sk = seq_lens ? max(0, min(ld_plan(seq_lens + b), Smax)) : Smax;
+struct BoundsTask {
+    const int *key_begin, *key_end, *seq_lens;
+    int4 *out;
+    int n, tiles, unit_rows, rows_per_kv, Sq, Smax, causal;
+};
+
+__device__ __forceinline__ void tile_bounds(const BoundsTask &p, int w, int lane) {
+    const int b = w / p.tiles, row0 = (w - b * p.tiles) * p.unit_rows, Sq = p.Sq;
+    const int rows = min(min(p.unit_rows, p.rows_per_kv - row0), Sq), i0 = row0 % Sq;
+    const int Sk = p.seq_lens ? max(0, min(ld_plan(p.seq_lens + b), p.Smax)) : p.Smax;
     const size_t at = (size_t)b * Sq;
+    constexpr int kTurns = kMostRows / 32;  // all loads in flight at once
+    int b0[kTurns], b1[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+        const int e = 32 * k + lane, i = i0 + e >= Sq ? i0 + e - Sq : i0 + e;
+        b0[k] = 0;
+        b1[k] = Sk;
+        if (e < rows) {
+            if (p.key_begin) b0[k] = ld_plan(p.key_begin + at + i);
+            if (p.key_end) b1[k] = ld_plan(p.key_end + at + i);
+        }
+    }
     int lo[2] = {0x7fffffff, 0x7fffffff}, hi[2] = {0, 0}, lo1 = 0, hi1 = Sk;  // [1]: past the border
     int runs[2] = {0, 0}, apart = 0;  // runs of rows that see keys, neighbours that do not touch
-    auto keys = [&](int i, int &b0, int &b1) {
-        b0 = key_begin ? max(ld_plan(key_begin + at + i), 0) : 0;
-        b1 = key_end ? min(ld_plan(key_end + at + i), Sk) : Sk;
-        if (causal) b1 = min(b1, Sk - Sq + i + 1);
-    };
-    for (int e = lane; e < rows; e += 32) {
-        const int past = i0 + e >= Sq, i = i0 + e - (past ? Sq : 0);
-        int b0, b1, c0 = 0, c1 = 0;
-        keys(i, b0, b1);
-        if (e > 0 && i > 0) keys(i - 1, c0, c1);  // the row before
-        if (b0 < b1) {
-            lo[past] = min(lo[past], b0);
-            hi[past] = max(hi[past], b1);
+    int last0 = 0, last1 = 0;         // the keys of the row before this turn's
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+        const int e = 32 * k + lane, past = i0 + e >= Sq, i = past ? i0 + e - Sq : i0 + e;
+        const int x0 = max(b0[k], 0);
+        int x1 = min(b1[k], Sk);
+        if (p.causal) x1 = min(x1, Sk - Sq + i + 1);
+        int c0 = __shfl_up_sync(0xffffffffu, x0, 1), c1 = __shfl_up_sync(0xffffffffu, x1, 1);  // the row before
+        if (lane == 0) c0 = last0, c1 = last1;
+        if (i == 0) c1 = c0;  // (none in this part)
+        last0 = __shfl_sync(0xffffffffu, x0, 31);
+        last1 = __shfl_sync(0xffffffffu, x1, 31);
+        if (e >= rows) continue;
+        if (x0 < x1) {
+            lo[past] = min(lo[past], x0);
+            hi[past] = max(hi[past], x1);
             if (c0 >= c1)
                 ++runs[past];
             else
-                apart |= max(b0, c0) > min(b1, c1);
+                apart |= max(x0, c0) > min(x1, c1);
         }
-        lo1 = max(lo1, b0);
-        hi1 = min(hi1, b1);
+        lo1 = max(lo1, x0);
+        hi1 = min(hi1, x1);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -70,10 +84,9 @@ __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
     apart = __any_sync(0xffffffffu, apart);
     lo1 = __reduce_max_sync(0xffffffffu, lo1);
     hi1 = __reduce_min_sync(0xffffffffu, hi1);
-    if (lane != 0) return;
     const int a = min(lo[0], lo[1]), z = max(hi[0], hi[1]);
     if (z <= a) {
-        out[2 * w] = out[2 * w + 1] = make_int4(0, 0, 0, 0);
+        if (lane == 0) p.out[2 * w] = p.out[2 * w + 1] = make_int4(0, 0, 0, 0);
         return;
     }
     int h0 = 0, h1 = 0;
@@ -83,20 +96,43 @@ __global__ void __launch_bounds__(256) mod_bounds_kernel(const int *key_begin,
     }
     // blocks from the first key's on, less whole ones of the hole (as the attention kernel walks them)
     const int base = a / kBlock * kBlock, skip = h1 > h0 ? (h1 - base) / kBlock - (h0 - base + kBlock - 1) / kBlock : 0;
-    out[2 * w] = make_int4(a, z, lo1, hi1);
-    out[2 * w + 1] = make_int4(h0, h1, (z - base + kBlock - 1) / kBlock - max(skip, 0),
-                             runs[0] <= 1 && runs[1] <= 1 && !apart && h1 <= h0);
+    const int blocks = (z - base + kBlock - 1) / kBlock - max(skip, 0);
+    if (lane == 0) {
+        p.out[2 * w] = make_int4(a, z, lo1, hi1);
+        p.out[2 * w + 1] = make_int4(h0, h1, blocks, runs[0] <= 1 && runs[1] <= 1 && !apart && h1 <= h0);
+    }
+}
+
+__global__ void __launch_bounds__(256) mod_bounds_kernel(const BoundsTask p) {
+    pdl_wait();
+    pdl_trigger();
+    const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (w < p.n) tile_bounds(p, w, threadIdx.x & 31);
 }
 
 // The units, longest first: a counting sort of the tiles by their key blocks (in steps of 2^shift blocks),
-// every tile standing for its sequence's kv heads. The order of equal ones is arbitrary; no result depends
-// on it.
-__global__ void __launch_bounds__(1024) mod_order_kernel(const int4 *bounds, int *order, int n,
-                                                         int tiles, int hkv, int shift) {
+// every tile standing for its sequence's kv heads. Up to kRanked tiles are ranked by comparing all of them, which
+// leaves equal ones in their own order (a launch's time then repeats, too); among more, equal ones come as
+// they happen to. No result depends on the order.
+constexpr int kRanked = 1024;
+__global__ void __launch_bounds__(1024) mod_order_kernel(const int4 *bounds, int *order, int n, int tiles, int hkv, int shift) {
     __shared__ int count[kBins], warp_sum[32];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto place = [&](int w, int at) {
+        const int b = w / tiles, tile = w - b * tiles;
+        for (int h = 0; h < hkv; ++h) order[at + h] = (b * hkv + h) * tiles + tile;
+    };
+    if (n <= kRanked) {
+        const int mine = tid < n ? ld_plan(bounds + 2 * tid + 1).z : 0;
+        if (tid < n) count[tid] = mine;
+        __syncthreads();
+        int rank = 0;
+        for (int w = 0; w < n; ++w) rank += count[w] > mine || (count[w] == mine && w < tid);
+        if (tid < n) place(tid, rank * hkv);
+        return;
+    }
     for (int i = tid; i < kBins; i += 1024) count[i] = 0;
     __syncthreads();
     // bin 0: the longest
@@ -119,10 +155,7 @@ __global__ void __launch_bounds__(1024) mod_order_kernel(const int4 *bounds, int
     count[2 * tid] = before;
     count[2 * tid + 1] = before + c0;
     __syncthreads();
-    for (int w = tid; w < n; w += 1024) {
-        const int at = atomicAdd(&count[bin(w)], hkv), b = w / tiles, tile = w - b * tiles;
-        for (int h = 0; h < hkv; ++h) order[at + h] = (b * hkv + h) * tiles + tile;
-    }
+    for (int w = tid; w < n; w += 1024) place(w, atomicAdd(&count[bin(w)], hkv));
 }
 
 // Token i of document [s, e) sees keys [s, i] and the document's first prefix tokens (causal), or the
@@ -178,14 +211,14 @@ static int launch(void (*kern)(KArgs...), unsigned grid, unsigned block, cudaStr
 extern "C" int ts_launch_mod_bounds(const fa_problem *P, void *stream) {
     const int tiles = ts_tc_ctas_per_split(P) / P->Hkv, n = P->Hkv / P->hkv_local * tiles;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int4 *bounds = reinterpret_cast<int4 *>(P->bounds);
-    const int rc = ts::launch(ts::mod_bounds_kernel, (unsigned)((n + 7) / 8), 256, st, P->key_begin, P->key_end,
-                              P->paged ? P->seq_lens : nullptr, bounds, n, tiles, ts_tc_unit_rows(P),
-                              P->Hq / P->Hkv * P->Sq, P->Sq, P->Sk, P->causal);
+    const ts::BoundsTask task = {P->key_begin, P->key_end, P->paged ? P->seq_lens : nullptr,
+                                 reinterpret_cast<int4 *>(P->bounds), n, tiles, ts_tc_unit_rows(P),
+                                 P->Hq / P->Hkv * P->Sq, P->Sq, P->Sk, P->causal};
+    const int rc = ts::launch(ts::mod_bounds_kernel, (unsigned)((n + 7) / 8), 256, st, task);
     if (rc != ATTN_OK || !P->order) return rc;
     int shift = 0;
     while (((P->Sk - 1) / ts::kBlock + 1) >> shift >= ts::kBins) ++shift;
-    return ts::launch(ts::mod_order_kernel, 1u, 1024, st, bounds, P->order, n, tiles, P->hkv_local, shift);
+    return ts::launch(ts::mod_order_kernel, 1u, 1024, st, task.out, P->order, n, tiles, P->hkv_local, shift);
 }
 
 extern "C" int ts_launch_mask_ranges(const int *cu_docs, const int *prefix, int n_docs, int S, int causal, int window,
