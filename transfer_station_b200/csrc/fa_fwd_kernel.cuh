@@ -38,6 +38,19 @@
 // (in exp2 units); otherwise the old max stays the reference and P may exceed 1 by at most
 // that factor. The quotient acc/l is the same mathematical value; this skips most O
 // rescales (TMEM round trips).
+//
+// Modified scores (MOD): z = cap tanh(s / cap) - slope |distance|, keys within a row's range. What is different:
+//   * The elementwise work bounds these forms, not the MMAs: a capped score takes 2.5 packed FMAs of a
+//     polynomial and a compare more than a plain one. Up to a cap of 52 the reference is the fixed cap_ref, so
+//     a capped block needs no maximum, no rescale and no second look. 32 / 8 heads, 4,096 tokens, D = 128, causal, bf16
+//     out: plain 152 us, ranges 147, bias 162, cap 190, cap and bias 226.
+//   * Units whose key ranges or lengths differ are sorted by their blocks, longest first (fa_mod.cu), and walked
+//     in alternating directions; blocks that none of a unit's rows sees are not walked, in front, behind or
+//     between the keys of two query heads. Nine documents in 6,007 tokens: 274 us in the units' own order, 187
+//     sorted, 147 with partly seen blocks kept in registers. An item costs about 6 us beside its blocks
+//     (Q, the first block's maximum, the output), 1.9 us each.
+//   * Slots that no row of the unit sees may hold anything: their V rows are zeroed in shared memory. Where the
+//     rows' ranges leave no gap (fa_mod.cu says so) only the first and last block need a look.
 #pragma once
 
 #include <cuda.h>

@@ -27,12 +27,14 @@
 // shared memory (2 bytes an element: 92 of the 128 bytes a clock) and 128 rows of queries. fp16 rather than
 // bf16: the weights keep 11 bits, and Q, 8 bits wide, is exact after a power-of-two scale per row.
 //
-// Work split. Tiles of kTile keys of all (sequence, kv head, row block) units form one list; CTA c of G
-// takes the c-th G-th of it, whatever the lengths are, so a ragged batch stays balanced without the host
-// knowing a length. A unit cut between CTAs leaves (m, l, acc) partials, merged by kv4_combine.
-// One producer warp per CTA streams tiles into a ring of shared-memory stages with untiled bulk copies;
-// four consumer warps take 32 keys of each tile, each with its own running maximum and accumulator, merged
-// in shared memory at a unit's end.
+// Work split: rows_plan.cuh. One producer warp per CTA streams tiles into a ring of shared-memory stages (codes by
+// TMA, scales by untiled bulk copies); four consumer warps take 32 keys of each tile, each with its own
+// running maximum and accumulator, merged in shared memory at a unit's end.
+//
+// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 128 us, 4 of 131,072 123 us, each 571 MB
+// of cache, 4.5 TB/s; streaming the same tiles without arithmetic takes 96 us, the arithmetic without the
+// streaming 124. 9 to 16 rows of a kv head in one column pair against two passes of 8: 238 us and 246 (64
+// sequences of 8,192 keys, 16 rows), D = 64 136 and 169.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
