@@ -160,3 +160,17 @@ def test_sorted_paged_batch(cuda_dev):
     seen = visible(B, Sq, lens, 1, Sk=Sk, dev=cuda_dev)
     ref, tol = attend(q, k, v, seen, lens, 0.0, sl)
     check(o, ref, tol)
+
+
+def test_what_a_fresh_scratch_block_holds(cuda_dev):
+    """Small numbers in a scratch block's first words are no report of a call, whichever call it is."""
+    B, Hq, Hkv, Sk, D = 1, 4, 1, 40, 64
+    q, k, v = inputs(B, Hq, Hkv, 1, Sk, D, cuda_dev, 2)
+    mod = ts.attn_mod(softcap=30.0)
+    scr = scratch(D, cuda_dev)
+    words = scr[:256].view(torch.int32)
+    want = call(q, k, v, mod, scr=scr)
+    for gen in range(1, 400):  # (calls of one process are numbered: words that run ahead of them by any amount)
+        words.copy_(torch.arange(64, dtype=torch.int32, device=cuda_dev) * 0 + 4)
+        words[3] = gen * 2
+        assert torch.equal(call(q, k, v, mod, scr=scr), want)

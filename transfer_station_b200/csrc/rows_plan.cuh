@@ -311,7 +311,9 @@ template <int TILE, int D, int ROWS>
 int plan_rows(RowsParams &p, int fit, int part_rows, int &ctas) {
     if (fit < 0) return ATTN_ERR_CUDA;
     p.row_blocks = (p.group * p.Sq + ROWS - 1) / ROWS;
-    p.gen = ts_next_status_gen();
+    // (spread over 32 bits, an odd factor: what a fresh scratch block happens to hold, small numbers mostly, must not
+    // pass for this call's reports)
+    p.gen = ts_next_status_gen() * 2654435761u;
     const long long units = (long long)p.B * p.Hkv * p.row_blocks, tiles = ((long long)p.Sk + TILE - 1) / TILE;
     long long n = (long long)ts_num_sms() * fit;
     if (n > part_rows / (2 * ROWS)) n = part_rows / (2 * ROWS);
