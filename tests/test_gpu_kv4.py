@@ -430,3 +430,29 @@ def test_streams_with_their_own_scratch(cuda_dev):
             run(q, pl, table, total, ln, P, None, torch.float32, dev, scrs[n], outs[n], st[n])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("Hq,Sq", [(4, 3), (16, 2), (8, 20), (2, 40)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_unseen_slots_between_ranges(cuda_dev, Hq, Sq, D):
+    """Rows that see ranges far apart: the slots between, before and behind them hold NaN scales and any code."""
+    dev, lens, Hkv, P = cuda_dev, [1200, 700], 2, 32
+    B = len(lens)
+    pl, table, total, k, v = cache(B, Hkv, D, lens, P, dev, Sq)
+    i = torch.arange(Sq, dtype=torch.int32, device=dev)
+    begin = torch.stack([101 + 190 * (i % 5), 333 - 7 * (i % 3)]).contiguous()
+    end = begin + torch.stack([13 + i % 9, 2 + 0 * i])
+    seen = visible(B, Sq, lens, 0, begin, end, k.shape[2], dev)
+    for b, n in enumerate(lens):
+        t = torch.arange(n, device=dev)
+        gone = ~seen[b, :, :n].any(0)
+        pg, row = table[b].long().clamp(min=0)[t // P][gone], (t % P)[gone]
+        pl[1][pg, :, row] = 0x7F
+        pl[3][pg, :, row] = 0xFF
+    g = torch.Generator(device=dev)
+    g.manual_seed(8)
+    q = torch.randn(B, Hq, Sq, D, generator=g, device=dev).bfloat16()
+    o, scr = run(q, pl, table, total, lens, P, ts.attn_mod(key_begin=begin, key_end=end), torch.float32, dev)
+    assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
+    ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -10, p_abs=2.0 ** -26)
+    check(o, ref, tol)

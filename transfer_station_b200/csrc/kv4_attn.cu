@@ -445,16 +445,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                         for (int b = 0; b < kSlabs; ++b) less_bias(s[b][n], 16.f * b, at, near[n], slope2[n]);
                     }
                 }
+                uint32_t seen[kSlabs];  // bits 0 to 3: some row sees key 2t, 2t + 1, 2t + 8, 2t + 9 of the slab
                 if (!whole) {
 #pragma unroll
-                    for (int b = 0; b < kSlabs; ++b)
+                    for (int b = 0; b < kSlabs; ++b) {
+                        bool any[2] = {false, false};
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int key = key0 + 16 * b + g + 8 * (e >> 1);
-                                if (key < lo[n][e & 1] || key >= hi[n][e & 1]) s[b][n][e] = -INFINITY;
+                                const bool in = key >= lo[n][e & 1] && key < hi[n][e & 1];
+                                any[e >> 1] |= in;
+                                if (!in) s[b][n][e] = -INFINITY;
                             }
+                        seen[b] = 0;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t lanes = __ballot_sync(0xffffffffu, any[h]) >> (8 * t);
+                            seen[b] |= ((lanes & 0x0fu) ? 1u << (2 * h) : 0u) | ((lanes & 0xf0u) ? 2u << (2 * h) : 0u);
+                        }
+                    }
                 }
                 bool above = false;
 #pragma unroll
@@ -536,8 +547,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                         // what an unseen slot holds may be any byte, a NaN scale among them: it becomes zero
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int key = key0 + 16 * b + 2 * t + (j & 1) + 8 * (j >> 1);
-                            if (key < span.lo || key >= span.hi)
+                            if (!((seen[b] >> j) & 1u))
 #pragma unroll
                                 for (int w = 0; w < GROUPS / 2; ++w) sc[j >> 1][w] &= (j & 1) ? 0x00ff00ffu : 0xff00ff00u;
                         }
