@@ -28,7 +28,7 @@
 // bf16: the weights keep 11 bits, and Q, 8 bits wide, is exact after a power-of-two scale per row.
 //
 // Work split: rows_plan.cuh. One producer warp per CTA streams tiles into a ring of shared-memory stages (codes by
-// TMA, scales by untiled bulk copies); four consumer warps take 32 keys of each tile, each with its own
+// TMA, scales by 16-byte copies); four consumer warps take 32 keys of each tile, each with its own
 // running maximum and accumulator, merged in shared memory at a unit's end.
 //
 // Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 128 us, 4 of 131,072 123 us, each 571 MB
@@ -40,6 +40,8 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "attn_kv4.h"
 #include "fa_launch.h"
@@ -56,11 +58,24 @@ constexpr int kSlabs = 2;        // 16-key MMA rows of a warp and tile
 constexpr int kThreads = 32 * (kWarps + 1);
 
 constexpr float kHead = 4.f, kMost = 7.f;  // see the weights
+// With small pages the copy engine is bound by the number of copies, and a page's 64 bytes of scales take as
+// long as its codes: up to this page size the producer's lanes fetch them. 64 sequences of 4,096 keys (32 / 8 heads,
+// D = 128), by the engine and by the lanes: pages of 8 149 and 122 us, 16 93 and 83, 32 76 and 75, 64 70 and 71.
+constexpr int kSmallPage = 32;
 
 struct Kv4Params : RowsParams {
     const uint8_t *kc, *ks, *vc, *vs;
     float cap_in, cap_out, tanh_k[5];
 };
+
+// 16 bytes from global to shared memory, asynchronously; and one arrival at a barrier once this thread's copies so
+// far have landed.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 
 template <int D, int NT>
 struct Kv4Config {
@@ -150,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
         for (int s = 0; s < C::NS; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), 1 + (p.page_size <= kSmallPage ? 32 : 0));  // (each producer lane's scales)
             mbar_init(empty(s), kWarps);
         }
         fence_mbar_init();
@@ -174,62 +189,81 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         int st = 0;                                  // next stage, and the round of the ring it is in
         uint32_t round = 0;
         bool ok = true;
-        while (left > 0 && ok) {
-            const Span sp = seq_span<kTile>(p, b);
-            const int len = sp.len, nt = sp.nt;
-            const int kvh = u / p.row_blocks;
-            const int used = (len + P - 1) / P;
-            const int *table = p.block_table + (size_t)b * p.max_pages;
-            const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
-            // chunk ids (a chunk: `rows` keys) of the next 32 chunks, one a lane
-            int win = -1, id = -1;
-            for (int i = tile; i < end && ok; ++i) {
-                const int c0 = (sp.t0 + i) * per_tile;
-                if (win < 0 || c0 + per_tile > win + 32) {
-                    win = c0;
-                    const long long key = (long long)(c0 + lane) * rows;
-                    const int page = (int)(key / P);
-                    id = -1;
-                    if (key < len && page < used) {
-                        id = ld_plan(table + page);
-                        if (id < 0 || id >= p.num_pages) {
-                            report_pending(p, kDevErrBadPage);
-                            id = -1;
+        auto produce = [&](auto small_pages) {
+            constexpr bool small = decltype(small_pages)::value;
+            while (left > 0 && ok) {
+                const Span sp = seq_span<kTile>(p, b);
+                const int len = sp.len, nt = sp.nt;
+                const int kvh = u / p.row_blocks;
+                const int used = (len + P - 1) / P;
+                const int *table = p.block_table + (size_t)b * p.max_pages;
+                const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
+                // chunk ids (a chunk: `rows` keys) of the next 32 chunks, one a lane
+                int win = -1, id = -1;
+                for (int i = tile; i < end && ok; ++i) {
+                    const int c0 = (sp.t0 + i) * per_tile;
+                    if (win < 0 || c0 + per_tile > win + 32) {
+                        win = c0;
+                        const long long key = (long long)(c0 + lane) * rows;
+                        const int page = (int)(key / P);
+                        id = -1;
+                        if (key < len && page < used) {
+                            id = ld_plan(table + page);
+                            if (id < 0 || id >= p.num_pages) {
+                                report_pending(p, kDevErrBadPage);
+                                id = -1;
+                            }
                         }
                     }
-                }
-                if (round > 0) ok = ring_wait(empty(st), (round - 1) & 1u, abort_flag, p, kDevErrTimeoutKV);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const int my_id = __shfl_sync(0xffffffffu, id, (c0 - win + lane) & 31);
-                const bool mine = lane < per_tile && my_id >= 0;
-                const int n = __popc(__ballot_sync(0xffffffffu, mine));
-                const uint32_t code_bytes = (uint32_t)(rows * (D / 2)), scale_bytes = (uint32_t)(rows * GROUPS);
-                if (lane == 0) mbar_expect_tx(full(st), (uint32_t)n * 2u * (code_bytes + scale_bytes));
-                __syncwarp();
-                if (mine) {
-                    const int row0 = (int)(((long long)(c0 + lane) * rows) % P);
-                    const int plane = my_id * p.Hkv + kvh;
-                    const size_t at = (size_t)plane * P + row0;  // row of the scale pools
+                    if (round > 0) ok = ring_wait(empty(st), (round - 1) & 1u, abort_flag, p, kDevErrTimeoutKV);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const int my_id = __shfl_sync(0xffffffffu, id, (c0 - win + lane) & 31);
+                    const bool mine = lane < per_tile && my_id >= 0;
+                    const int n = __popc(__ballot_sync(0xffffffffu, mine));
+                    const uint32_t code_bytes = (uint32_t)(rows * (D / 2)), scale_bytes = (uint32_t)(rows * GROUPS);
                     const uint32_t dst = base + st * C::STAGE, bar = full(st);
-                    tma_load_3d(dst + lane * code_bytes, &tmK, bar, 0, row0, plane);
-                    bulk_load(dst + C::K_SCALES + lane * scale_bytes, p.ks + at * GROUPS, scale_bytes, bar);
-                    tma_load_3d(dst + C::V_CODES + lane * code_bytes, &tmV, bar, 0, row0, plane);
-                    bulk_load(dst + C::V_SCALES + lane * scale_bytes, p.vs + at * GROUPS, scale_bytes, bar);
+                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)n * 2u * (code_bytes + (small ? 0u : scale_bytes)));
+                    __syncwarp();
+                    if (mine) {
+                        const int row0 = (int)(((long long)(c0 + lane) * rows) % P);
+                        const int plane = my_id * p.Hkv + kvh;
+                        const size_t at = ((size_t)plane * P + row0) * GROUPS;  // in the scale pools
+                        tma_load_3d(dst + lane * code_bytes, &tmK, bar, 0, row0, plane);
+                        if (!small) bulk_load(dst + C::K_SCALES + lane * scale_bytes, p.ks + at, scale_bytes, bar);
+                        tma_load_3d(dst + C::V_CODES + lane * code_bytes, &tmV, bar, 0, row0, plane);
+                        if (!small) bulk_load(dst + C::V_SCALES + lane * scale_bytes, p.vs + at, scale_bytes, bar);
+                    }
+                    if constexpr (small) {  // the scales in pieces of 16 bytes
+                        constexpr int KEYS = 16 / GROUPS, PIECES = kTile / KEYS;  // keys of a piece, pieces of a pool and tile
+                        const int key = (lane & (PIECES - 1)) * KEYS;
+                        const int sid = __shfl_sync(0xffffffffu, id, (c0 - win + key / rows) & 31);
+                        if (sid >= 0) {
+                            const int row = (int)(((long long)c0 * rows + key) % P);
+                            const size_t at = ((size_t)(sid * p.Hkv + kvh) * P + row) * GROUPS;
+                            if (PIECES == 32 || lane < PIECES) copy16(dst + C::K_SCALES + key * GROUPS, p.ks + at);
+                            if (PIECES == 32 || lane >= PIECES) copy16(dst + C::V_SCALES + key * GROUPS, p.vs + at);
+                        }
+                        copy_arrive(bar);
+                    }
+                    __syncwarp();
+                    if (++st == C::NS) {
+                        st = 0;
+                        ++round;
+                    }
                 }
-                __syncwarp();
-                if (++st == C::NS) {
-                    st = 0;
-                    ++round;
+                left -= end - tile;
+                tile = 0;
+                if (++u == units) {
+                    u = 0;
+                    ++b;
                 }
             }
-            left -= end - tile;
-            tile = 0;
-            if (++u == units) {
-                u = 0;
-                ++b;
-            }
-        }
+        };
+        if (P <= kSmallPage)
+            produce(std::true_type{});
+        else
+            produce(std::false_type{});
         // copies in flight land before the CTA exits: the last issue of each stage
         for (int j = 0; j < C::NS; ++j) {
             volatile int never = 0;
