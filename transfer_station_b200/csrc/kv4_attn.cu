@@ -20,7 +20,7 @@
 //     four elements in the halves of a register (V): the operand layouts without a permute. The code tiles
 //     come by TMA with the 64-byte (D = 64: 32-byte) swizzle, so the eight rows of a matrix lie in
 //     different banks.
-// Dequantising everything to fp16 with the scales took 131 us where this takes 129 us (B = 64,
+// Dequantising everything to fp16 with the scales took 131 us where this took 129 us (B = 64,
 // Sk = 8192, 32/8 heads, D = 128; streaming the same bytes without arithmetic: 96).
 // Keys are the M side of mma.m16n8k16 and the query rows of a kv head the N side: up to 8 rows cost one
 // MMA per 16 keys x 16 elements, with no padding rows. tcgen05 would need the operand tile written back to
@@ -31,7 +31,7 @@
 // TMA, scales by 16-byte copies); four consumer warps take 32 keys of each tile, each with its own
 // running maximum and accumulator, merged in shared memory at a unit's end.
 //
-// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 128 us, 4 of 131,072 123 us, each 571 MB
+// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 126 us, 4 of 131,072 122 us, each 571 MB
 // of cache, 4.5 TB/s; streaming the same tiles without arithmetic takes 96 us, the arithmetic without the
 // streaming 124. 9 to 16 rows of a kv head in one column pair against two passes of 8: 238 us and 246 (64
 // sequences of 8,192 keys, 16 rows), D = 64 136 and 169.
