@@ -77,3 +77,8 @@ def test_no_b200_is_reported(built_lib):
     assert contiguous(mod(softcap=30.0)) == ts.ATTN_ERR_NOT_SM100
     assert contiguous(None) == ts.ATTN_ERR_NOT_SM100
     assert paged(mod(causal=1)) == ts.ATTN_ERR_NOT_SM100
+
+
+def test_more_kv_heads_than_heads(built_lib):
+    """Refused before the product of batch and kv heads is formed."""
+    assert contiguous(mod(softcap=30.0), B=1 << 20, Hq=8, Hkv=1 << 20) == ts.ATTN_ERR_ARGS

@@ -356,13 +356,13 @@ static int ts_run_mod(fa_problem *p, void *scratch, void *stream) {
 
 int attn_flash_mod_stream(const uint16_t *Q, const uint16_t *K, const uint16_t *V, void *O, int out_dtype, int B,
                           int Hq, int Hkv, int Sq, int Sk, int D, const attn_mod *mod, void *scratch, void *stream) {
-    if (!O || (out_dtype != ATTN_OUT_F32 && out_dtype != ATTN_OUT_BF16) || B < 1 || Hq < 1 || Hkv < 1)
+    if (!O || (out_dtype != ATTN_OUT_F32 && out_dtype != ATTN_OUT_BF16) || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0)
         return ATTN_ERR_ARGS;
     if ((long long)B * Hq > 0x7fffffffLL) return ATTN_ERR_ARGS;
     fa_problem p;
     ts_fill(&p, Q, K, V, B * Hq, B * Hkv, Sq, Sk, D < 1 ? 1 : D, 0, 0);
     int rc = ts_set_mod(&p, mod, Hkv);
-    if (rc == ATTN_ERR_ARGS || Hq % Hkv != 0) return ATTN_ERR_ARGS;
+    if (rc == ATTN_ERR_ARGS) return rc;
     const int valid = ts_validate(Q, K, V, B * Hq, B * Hkv, Sq, Sk, D, scratch);
     if (valid == ATTN_ERR_ARGS) return valid;
     if (rc != ATTN_OK) return rc;
