@@ -141,9 +141,9 @@ struct TcConfig {
     static constexpr int OSTAGE = 32 * 32 * 4;
     static constexpr int NOSTAGE = NQT == 2 ? 8 : 0;  // one-tile instances keep per-row stores
     static constexpr int SMEM = 1024 + NQT * QTILE + NS * KVTILE + NOSTAGE * OSTAGE + NBAR * 8 + 16;
-    static constexpr int SEEN_WORDS = 2 * 4 * 4;  // MOD: two buffers of four warps' 128 key bits
+    static constexpr int SEEN_WORDS = 2 * 4 * 4;  // MOD: two buffers of four warps' 128 key bits, and their barrier
     static constexpr int smem_bytes(bool paged, bool mod = false) {
-        return SMEM + (paged ? PID_WIN * 4 : 0) + (mod ? SEEN_WORDS * 4 : 0);
+        return SMEM + (paged ? PID_WIN * 4 : 0) + (mod ? SEEN_WORDS * 4 + 8 : 0);
     }
     static_assert(smem_bytes(true, true) <= 227 * 1024, "shared memory per CTA");
     static constexpr int THREADS = 128 + 128 * NQT;
@@ -161,11 +161,6 @@ __device__ __forceinline__ uint32_t span_bits(int a, int b) {
     a = max(a, 0);
     b = min(b, 32);
     return b > a ? (0xffffffffu >> (32 - (b - a))) << a : 0u;
-}
-
-// Barrier among `count` threads of the CTA (id 0 is __syncthreads').
-__device__ __forceinline__ void named_sync(int id, int count) {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
 // Waits without honouring the abort flag: used only at teardown, to let TMA copies and MMAs
@@ -223,6 +218,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *pid_win = reinterpret_cast<int *>(tmem_slot + 4);  // paged K/V: C::PID_WIN page ids
     uint32_t *seen_bits = reinterpret_cast<uint32_t *>(tmem_slot + 4 + (PAGED ? C::PID_WIN : 0));  // MOD
+    const uint32_t seen_bar = smem_u32(seen_bits + C::SEEN_WORDS);  // MOD: the four warps' words are there
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -387,6 +383,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             mbar_init(p_full(t), 128);
             mbar_init(o_full(t), 1);
         }
+        if constexpr (MOD != 0) mbar_init(seen_bar, 4);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -1203,8 +1200,8 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 bool keep = key0 + r >= it.ulo && key0 + r < it.uhi;
                 if (!it.solid) {
                     // the union of both tiles' rows as 128 bits, a word per 32 keys
-                    uint32_t *buf = seen_bits + 16 * (seen_turn & 1);
-                    ++seen_turn;
+                    const uint32_t turn = seen_turn++ & 1;
+                    uint32_t *buf = seen_bits + 16 * turn;
                     const int m0 = max(lo_b - key0, 0), m1 = min(hi_b - key0, kBN);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -1213,8 +1210,16 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                         const uint32_t all = __reduce_or_sync(0xffffffffu, w);
                         if (lane == 0) buf[4 * quad + k] = all;
                     }
-                    __syncwarp();
-                    named_sync(1, 128);  // two buffers: the next block's words never meet late readers
+                    // Two buffers: the next block's words never meet late readers. An mbarrier, because a warp that
+                    // gives up (a bad page aborts the CTA between two warps' polls) never arrives: the others'
+                    // wait sees the abort flag, as every wait here does.
+                    if (lane == 0) mbar_arrive(seen_bar);
+                    ok = mbar_wait(seen_bar, turn, abort_flag, p.status, kDevErrTimeoutS, p.gen);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) {
+                        tmem_wait_st();  // P's stores land before the CTA frees its TMEM
+                        break;
+                    }
                     const uint32_t any = buf[quad] | buf[4 + quad] | buf[8 + quad] | buf[12 + quad];
                     keep = (any >> lane) & 1u;
                 }
@@ -1223,7 +1228,10 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                     const int sV = (int)(iV % NS);
                     ok = mbar_wait(kv_full(sV), (iV / NS) & 1, abort_flag, p.status, kDevErrTimeoutKV, p.gen);
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!ok) {
+                        tmem_wait_st();
+                        break;
+                    }
                     if (!keep) {
 #pragma unroll
                         for (int b = 0; b < NBOX_D; ++b)
