@@ -1121,7 +1121,10 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                         }
                         const float rs = (acc0.x + acc1.x) + (acc0.y + acc1.y);
                         general = __any_sync(0xffffffffu, rs > kRedoSum);
-                        if (!general) l += rs;
+                        if (general)
+                            tmem_wait_st();  // the speculative P stores land before the exact ones
+                        else
+                            l += rs;
                         acc0 = acc1 = make_float2(0.f, 0.f);
                     } else {
 #pragma unroll
