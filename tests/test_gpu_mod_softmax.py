@@ -31,3 +31,26 @@ def test_maximum_moves_at_every_block(cuda_dev, Sq, D, bias, step):
     check(o, ref, tol)
     for _ in range(5):
         assert torch.equal(call(q, k, v, mod), o)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Sk,D,causal,cap,signs", [
+    (1, 4, 2, 300, 1500, 128, 1, 50.0, "-"),   # 216 log2 units of bias over the keys
+    (1, 4, 2, 300, 1500, 64, 0, 30.0, "-"),    # keys ahead of the query too
+    (2, 4, 1, 60, 1100, 128, 1, 20.0, "+-"),   # heads of either sign share a unit, and a warp
+    (1, 6, 2, 10, 3000, 64, 1, 50.0, "+-"),    # one row tile, keys in pieces
+    (1, 4, 2, 130, 1200, 64, 1, 200.0, "-"),   # a cap past the fixed reference
+    (1, 4, 2, 3, 1500, 128, 1, 50.0, "-"),     # the form for few rows
+    (1, 4, 2, 20, 1500, 36, 1, 50.0, "-"),     # the general form
+])
+def test_capped_scores_with_a_rising_bias(cuda_dev, B, Hq, Hkv, Sq, Sk, D, causal, cap, signs):
+    """Negative slopes: scores grow with the distance, past the cap and any fixed reference."""
+    q, k, v = inputs(B, Hq, Hkv, Sq, Sk, D, cuda_dev, Sq + D, 2.0)
+    sl = torch.full((Hq,), -0.1, device=cuda_dev)
+    if signs == "+-":
+        sl[::2] = 0.07
+    mod = ts.attn_mod(softcap=cap, causal=causal, slopes=sl)
+    o = call(q, k, v, mod)
+    seen = visible(B, Sq, [Sk] * B, causal, Sk=Sk, dev=cuda_dev)
+    ref, tol = attend(q, k, v, seen, [Sk] * B, cap, sl)
+    check(o, ref, tol)
+    assert torch.equal(call(q, k, v, mod), o)

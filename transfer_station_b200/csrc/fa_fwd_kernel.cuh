@@ -748,6 +748,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
         // MOD: this row's keys [lo, hi) and its query position; rows past the problem follow the last one.
         int lo = 0, hi = 0, qpos = 0, near = 0;
         float slope2 = 0.f;      // distance bias per key, log2 units
+        bool fixed = false;      // the warp's rows take the fixed reference
         int lo_b = 0, hi_b = 0;  // the keys of the row 128 further on (the unit's other tile)
         if constexpr (MOD != 0) {
             auto row_keys = [&](int row, int &first, int &end) {
@@ -769,7 +770,9 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 near = max(0, max(lo - qpos, qpos - (hi - 1)));
             }
             hi = min(hi, kb1);  // of this piece
-            if (kCap && p.cap_ref >= 0.f) m = p.cap_ref;
+            // (a bias that rises with the distance has no bound: such a warp's rows keep a running maximum)
+            fixed = kCap && p.cap_ref >= 0.f && (!kBias || __all_sync(0xffffffffu, slope2 >= 0.f));
+            if (fixed) m = p.cap_ref;
         }
         for (int j = 0; j < nblk; ++j) {
             if constexpr (MOD == 0) {
@@ -947,8 +950,9 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             // Modified scores. z = the modified score in log2 units; m is kept in the same units.
             //   none     no row of the warp sees a key of the block: P = 0
             //   fixed    capped scores lie within +-cap_out: up to cap_out = 75 (a cap of 52) the fixed
-            //            reference cap_ref keeps every P in [2^-100, 2^50], so there is no maximum, no
-            //            rescale and no second look -- one pass over the scores
+            //            reference cap_ref keeps P within 2^50, and a row's largest above 2^-100 (a bias
+            //            takes from every key but the nearest), so there is no maximum, no rescale and no
+            //            second look -- one pass over the scores
             //   spec     the plain kernel's speculation: P against the running max, redone when a row
             //            sum shows a max that moved by more than 2^kRescaleLog2
             //   general  two passes over the score tile: the max, then P
@@ -965,7 +969,6 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             const bool ahead = kBias && __all_sync(0xffffffffu, key0 + n0 >= qpos);
             const float bs = past ? slope2 : -slope2;
             const float b0 = kBias ? bs * (float)(key0 - (past ? qpos - near : qpos + near)) : 0.f;
-            const bool fixed = kCap && p.cap_ref >= 0.f;
             const bool spec = !kCap && full && (past || ahead) && __all_sync(0xffffffffu, m != -INFINITY);
             ok = mbar_wait(s_full(t), sp & 1, abort_flag, p.status, kDevErrTimeoutS, p.gen);
             ++sp;
@@ -978,7 +981,8 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 const float2 b02 = make_float2(b0 + add, b0 + add);
                 if constexpr (kCap) {
                     constexpr bool kRaw = decltype(raw_tag)::value;  // the polynomial takes raw scores
-                    const float2 in2 = make_float2(p.cap_in, p.cap_in);
+                    const float in = p.cap_ref >= 0.f ? 1.f : p.cap_in;  // (or it does for a running maximum too)
+                    const float2 in2 = make_float2(in, in);
                     const float2 end2 = kBias ? make_float2(0.f, 0.f) : add2;
                     float far = 0.f;
 #pragma unroll
