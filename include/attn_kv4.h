@@ -61,8 +61,8 @@ int attn_kv4_unpack_stream(const uint8_t *K_codes, const uint8_t *K_scales, cons
  * read as numbers, nor are table entries past its pages. A page
  * id outside the pool is reported by attn_flash_status; that sequence's rows are then undefined. At least
  * a million kv heads over all sequences are taken (their bookkeeping lies in scratch). Weights
- * are rounded to fp16 and dequantised elements are exact in fp16; scores, maxima, sums and accumulators
- * are fp32. */
+ * are rounded to fp16 once (11 bits down to 2^-26 of a row's largest, steps of 2^-36 of it below) and
+ * dequantised elements are exact in fp16; scores, maxima, sums and accumulators are fp32. */
 int attn_flash_kv4_stream(const uint16_t *Q, const uint8_t *K_codes, const uint8_t *K_scales,
                           const uint8_t *V_codes, const uint8_t *V_scales, const int *block_table,
                           const int *seq_lens, void *O, int out_dtype, int B, int Hq, int Hkv, int Sq, int D,

@@ -13,15 +13,14 @@
 //     and the scales stay off the elements: one accumulator per 32-element group gets -8 * 2^-24 *
 //     sum(Q over the group) added and is multiplied by the key's scale once. (e4m3 operands, whose
 //     nibbles need no more than a mask either and pair with Q split in two, ran at half this speed.)
-//   * Second product: one HFMA2 turns a masked pair into (n - 8) * 2^-9, normal numbers again, because the
-//     lost bits would not average out over long contexts. The value's scale goes into the weight, one
-//     fragment per group. (An MMA by -8 in place of the HFMA2s took 7% longer.)
+//   * Second product: one LOP3 and one HFMA2 turn a pair of nibbles into the values themselves, (n - 8) * s, exact.
+//     The weights stay as they are for every group. (The scale in the weight instead took 127 us where this takes
+//     133, but rounded twice, the second time below fp16's normal numbers: behind a key that holds most of the
+//     weight, or at small scales, the other keys' products lost their bits or were zero.)
 //   * ldmatrix gives each lane one 32-bit word of one group per key (K), and, transposed, two keys' same
 //     four elements in the halves of a register (V): the operand layouts without a permute. The code tiles
 //     come by TMA with the 64-byte (D = 64: 32-byte) swizzle, so the eight rows of a matrix lie in
 //     different banks.
-// Dequantising everything to fp16 with the scales took 131 us where this took 129 us (B = 64,
-// Sk = 8192, 32/8 heads, D = 128; streaming the same bytes without arithmetic: 96).
 // Keys are the M side of mma.m16n8k16 and the query rows of a kv head the N side: up to 8 rows cost one
 // MMA per 16 keys x 16 elements, with no padding rows. tcgen05 would need the operand tile written back to
 // shared memory (2 bytes an element: 92 of the 128 bytes a clock) and 128 rows of queries. fp16 rather than
@@ -31,10 +30,9 @@
 // TMA, scales by 16-byte copies); four consumer warps take 32 keys of each tile, each with its own
 // running maximum and accumulator, merged in shared memory at a unit's end.
 //
-// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 126 us, 4 of 131,072 122 us, each 571 MB
-// of cache, 4.5 TB/s; streaming the same tiles without arithmetic takes 96 us, the arithmetic without the
-// streaming 124. 9 to 16 rows of a kv head in one column pair against two passes of 8: 238 us and 246 (64
-// sequences of 8,192 keys, 16 rows), D = 64 136 and 169.
+// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 133 us, 4 of 131,072 130 us, each 571 MB
+// of cache, 4.3 TB/s; streaming the same tiles without arithmetic takes 96 us. 9 to 16 rows of a kv head in one
+// column pair (64 sequences of 8,192 keys, 16 rows): 236 us, D = 64 138; two passes of 8 took 246 and 169.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -57,7 +55,7 @@ constexpr int kWarps = 4;        // consumer warps, 32 keys of a tile each
 constexpr int kSlabs = 2;        // 16-key MMA rows of a warp and tile
 constexpr int kThreads = 32 * (kWarps + 1);
 
-constexpr float kHead = 4.f, kMost = 7.f;  // see the weights
+constexpr float kHead = 12.f, kMost = 15.f;  // see the weights
 // With small pages the copy engine is bound by the number of copies, and a page's 64 bytes of scales take as
 // long as its codes: up to this page size the producer's lanes fetch them. 64 sequences of 4,096 keys (32 / 8 heads,
 // D = 128), by the engine and by the lanes: pages of 8 149 and 122 us, 16 93 and 83, 32 76 and 75, 64 70 and 71.
@@ -115,16 +113,29 @@ __device__ __forceinline__ __half2 scales2(uint32_t bytes) {
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // fp16: n * 2^-24, n * 2^-20
-constexpr float kKeyUnit = 1.f / 16777216.f, kUnit = 1.f / 512.f;  // 2^-24 and 2^-9: what 1 stands for as a key, a value
+constexpr float kKeyUnit = 1.f / 16777216.f, kUnit = 1.f / 8.f;  // 2^-24 and 2^-3: what 1 stands for as a key, a value
 
-// A pair of masked nibbles -> (n - 8) * 2^-9, exact: times 2^15 (2^11), less 2^-6. (The constants as bits: the
-// conversion functions are not folded.)
-constexpr uint32_t kTwo15 = 0x78007800u, kTwo11 = 0x68006800u, kMinusEight = 0xa400a400u;
-__device__ __forceinline__ uint32_t centre_low(uint32_t x) {
-    return as_u32(__hfma2(as_half2(x & kLow), as_half2(kTwo15), as_half2(kMinusEight)));
+// A pair of nibbles (of two keys) -> the values (n - 8) * s over 8, exact: under an exponent of their own the nibbles
+// are 128 + n / 8 and 8 + n / 8, and (128 + n / 8) * s - 129 s is rounded once, to a number of 8 bits. s has 4
+// bits, so 129 s has 11 at most and 9 s has 8; with the largest scale, 448, all stay below 65504. (The constants as
+// bits: the conversion functions are not folded.)
+constexpr uint32_t k128 = 0x58005800u, k8 = 0x48004800u, kMinus129 = 0xd808d808u, kMinus9 = 0xc880c880u;
+struct ValueScales {  // s, -129 s, -9 s of two keys
+    __half2 s, low, high;
+    __device__ __forceinline__ explicit ValueScales(__half2 v)
+        : s(v), low(__hmul2(v, as_half2(kMinus129))), high(__hmul2(v, as_half2(kMinus9))) {}
+};
+// (x & mask) | exponent as one LOP3: written out, the compiler emits two with an immediate each
+__device__ __forceinline__ __half2 under(uint32_t x, uint32_t mask, uint32_t exponent) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(exponent));
+    return as_half2(r);
 }
-__device__ __forceinline__ uint32_t centre_high(uint32_t x) {
-    return as_u32(__hfma2(as_half2(x & kHigh), as_half2(kTwo11), as_half2(kMinusEight)));
+__device__ __forceinline__ uint32_t value_low(uint32_t x, const ValueScales &v) {
+    return as_u32(__hfma2(under(x, kLow, k128), v.s, v.low));
+}
+__device__ __forceinline__ uint32_t value_high(uint32_t x, const ValueScales &v) {
+    return as_u32(__hfma2(under(x, kHigh, k8), v.s, v.high));
 }
 
 // A slab's 16 rows of codes: lane (g, t) gets word t of every group of rows g and g + 8, or transposed the
@@ -512,9 +523,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                         above |= mx > most[n][c];
                     }
                 // A column's reference is its maximum less kHead when it was set, and moves only when a score
-                // exceeds it by kMost: weights reach from 2^kHead at the maximum up to 2^kMost, which times
-                // the largest scale (448) still is an fp16 number. (Until a column has seen a key, most is
-                // -inf and the reference 0.)
+                // exceeds it by kMost: weights reach from 2^kHead at the maximum up to 2^kMost, the upper end of fp16,
+                // and keep its 11 bits down to 2^-26 of the largest. (Until a column has seen a key, most is -inf and
+                // the reference 0.)
                 if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -589,16 +600,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 #pragma unroll
                     for (int w = 0; w < GROUPS; ++w) {
                         const uint32_t x = v0[w], y = v1[w], xs = x >> 8, ys = y >> 8;
-                        const uint32_t a0[4] = {centre_low(x), centre_high(x), centre_low(y), centre_high(y)};
-                        const uint32_t a1[4] = {centre_low(xs), centre_high(xs), centre_low(ys), centre_high(ys)};
-                        const __half2 s0 = scales2((w & 1) ? sc[0][w >> 1] >> 16 : sc[0][w >> 1] & 0xffffu);
-                        const __half2 s1 = scales2((w & 1) ? sc[1][w >> 1] >> 16 : sc[1][w >> 1] & 0xffffu);
+                        const ValueScales s0(scales2((w & 1) ? sc[0][w >> 1] >> 16 : sc[0][w >> 1] & 0xffffu));
+                        const ValueScales s1(scales2((w & 1) ? sc[1][w >> 1] >> 16 : sc[1][w >> 1] & 0xffffu));
+                        const uint32_t a0[4] = {value_low(x, s0), value_high(x, s0), value_low(y, s1), value_high(y, s1)};
+                        const uint32_t a1[4] = {value_low(xs, s0), value_high(xs, s0), value_low(ys, s1), value_high(ys, s1)};
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const uint32_t p0 = as_u32(__hmul2(as_half2(pf[n][0]), s0));
-                            const uint32_t p1 = as_u32(__hmul2(as_half2(pf[n][1]), s1));
-                            mma16816(acc[n][2 * w], a0, p0, p1);
-                            mma16816(acc[n][2 * w + 1], a1, p0, p1);
+                            mma16816(acc[n][2 * w], a0, pf[n][0], pf[n][1]);
+                            mma16816(acc[n][2 * w + 1], a1, pf[n][0], pf[n][1]);
                         }
                     }
                 }
