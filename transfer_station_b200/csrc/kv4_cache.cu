@@ -158,7 +158,8 @@ __device__ __forceinline__ uint2 quantise(uint4 ra, uint4 rb, __nv_fp8_storage_t
             const float2 x = unpack2(r[e]);
             a = fmaxf(a, fmaxf(fabsf(x.x), fabsf(x.y)));  // (a NaN leaves a as it is)
         }
-        a = fmaxf(a, __shfl_xor_sync(__activemask(), a, 1));  // (both lanes of the group are here)
+        // (both lanes of the group are here, other groups need not be)
+        a = fmaxf(a, __shfl_xor_sync(3u << (threadIdx.x & 30), a, 1));
         s8 = __nv_cvt_float_to_fp8(a / 7.0f, __NV_SATFINITE, __NV_E4M3);
         const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(s8, __NV_E4M3)));
         w[0] = w[1] = 0u;
