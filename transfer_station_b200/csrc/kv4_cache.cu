@@ -178,7 +178,7 @@ __device__ __forceinline__ uint2 quantise(uint4 ra, uint4 rb, __nv_fp8_storage_t
 }
 
 // |x| of the lower and the upper bf16 of a word as doubles, by moving bits: zero and subnormals come out below
-// 2^-126, which a sum of squares does not see.
+// 2^-126, which a sum of squares does not see, infinities and NaN as 2^128 and more.
 __device__ __forceinline__ double magnitude_lo(uint32_t w) {
     return __hiloint2double((int)((w & 0x7fffu) * 8192u + 0x38000000u), 0);
 }
@@ -305,6 +305,17 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(const ts_
                 const double r0 = (double)rsqrtf((float)v);
                 const double r1 = fma(0.5 * r0, fma(-v * r0, r0, 1.0), r0);
                 root = v > 1e-30 && v < 1e30 ? (float)r1 : (float)rsqrt(v);
+                // An infinity or a NaN stands in the sum as a number of 2^256 and more. The root over an infinity is
+                // zero, over a NaN it is one.
+                if (__any_sync(kFull, !(v < 1e30))) {
+                    uint32_t m = 0u;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+                    m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+                    for (int o = G / 2; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o, G));
+                    if (m >= 0x7f80u) root = m > 0x7f80u ? __uint_as_float(0x7fc00000u) : 0.f;
+                }
             } else {
                 float ss = 0.f;
 #pragma unroll
