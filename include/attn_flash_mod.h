@@ -17,7 +17,10 @@
  * Layouts are attn_flash's with batch folded into heads: Q [B*Hq][Sq][D], K and V [B*Hkv][Sk][D] bf16
  * bits, O [B*Hq][Sq][D] fp32 or bf16 bits. Tensors are contiguous and live on the current device.
  * P is rounded to bf16 for the second product (as flash.c rounds it); scores, maxima, sums and
- * accumulators are fp32. Asynchronous on `stream`; the same threads, scratch and status contract as
+ * accumulators are fp32. With a cap of up to 52, slopes of zero or more and more than 16 query rows of a kv
+ * head, weights are taken against a fixed score instead of a row's maximum, so they may reach 2^50, and a
+ * row's largest may be as low as 2^-100: values above 2^60 may then overflow, and values below 2^-20 lose bits in
+ * rows whose every score is near -softcap. Asynchronous on `stream`; the same threads, scratch and status contract as
  * attn_flash_stream. Calls can be captured into CUDA graphs; graphs that may run at the same time
  * need a scratch block each.
  */

@@ -54,3 +54,22 @@ def test_capped_scores_with_a_rising_bias(cuda_dev, B, Hq, Hkv, Sq, Sk, D, causa
     ref, tol = attend(q, k, v, seen, [Sk] * B, cap, sl)
     check(o, ref, tol)
     assert torch.equal(call(q, k, v, mod), o)
+
+
+@pytest.mark.parametrize("cap", [5.0, 15.0, 30.0, 37.0, 50.0, 52.0, 80.0])
+@pytest.mark.parametrize("size", [60, -20])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("bias", [0, 1])
+def test_values_of_any_size_under_a_cap(cuda_dev, cap, size, sign, bias):
+    """The documented range of values, where every score of a row lies near the cap (sign 1) or near its negative:
+    neither overflow nor what lies below fp32's normal numbers reaches the result."""
+    B, Hq, Hkv, Sq, Sk, D = 1, 4, 2, 200, 700, 64
+    q, k, v = inputs(B, Hq, Hkv, Sq, Sk, D, cuda_dev, 7)
+    v = (v.float() * 2.0 ** size).bfloat16()
+    q[..., 0], k[..., 0] = 32.0 * sign, 40.0  # raw scores of 160
+    sl = slopes_of(Hq, cuda_dev, 0.1) if bias else None
+    o = call(q, k, v, ts.attn_mod(softcap=cap, causal=1, slopes=sl))
+    seen = visible(B, Sq, [Sk], 1, Sk=Sk, dev=cuda_dev)
+    # (the bound with the values at one, scaled back: its smallest term is absolute)
+    ref, tol = attend(q, k, v.double() * 2.0 ** -size, seen, [Sk], cap, sl)
+    check(o.double() * 2.0 ** -size, ref, tol)
