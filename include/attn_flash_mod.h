@@ -56,7 +56,9 @@ int attn_flash_mod_stream(const uint16_t *Q, const uint16_t *K, const uint16_t *
 /* Attention over a paged K/V cache: attn_flash_paged_stream's pools, tables and limits (D a multiple
  * of 8 up to 128), with modified scores and a choice of output type. A sequence's key axis is its
  * seq_lens entry, so pos_i = seq_lens[b] - Sq + i. Rows of a page at or past the sequence's end are
- * not read as numbers. */
+ * not read as numbers. Of a sequence's block table the entries of the pages from the first key that any of its
+ * queries sees to the last are read, both ends rounded outwards to 128 keys; before and behind it may hold
+ * anything. An entry read that names no page of the pool is reported by attn_flash_status. */
 int attn_flash_mod_paged_stream(const uint16_t *Q, const uint16_t *K_pages, const uint16_t *V_pages,
                                 const int *block_table, const int *seq_lens, void *O, int out_dtype, int B, int Hq,
                                 int Hkv, int Sq, int D, const attn_mod *mod, int page_size, int num_pages,

@@ -58,8 +58,9 @@ int attn_kv4_unpack_stream(const uint8_t *K_codes, const uint8_t *K_scales, cons
  * [0, max_pages * page_size]; none: zero rows), its queries are its last Sq positions. mod (may be NULL)
  * as in attn_flash_mod_paged_stream: cap, bias, key ranges and causality over the sequence's keys. Rows
  * of a page past the sequence's end, and keys that no row of a unit sees (here up to 16 rows of a kv head), are not
- * read as numbers, nor are table entries past its pages. A page
- * id outside the pool is reported by attn_flash_status; that sequence's rows are then undefined. At least
+ * read as numbers. Of its block table the entries of the pages from the first key that any of its queries sees to
+ * the last are read (with more than 16 positions those of all its keys). A page
+ * id outside the pool there is reported by attn_flash_status; that sequence's rows are then undefined. At least
  * a million kv heads over all sequences are taken (their bookkeeping lies in scratch). Weights
  * are rounded to fp16 once (11 bits down to 2^-26 of a row's largest, steps of 2^-36 of it below) and
  * dequantised elements are exact in fp16; scores, maxima, sums and accumulators are fp32. */

@@ -459,7 +459,12 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
             if (it.nblk == 0) continue;
             const int kv = it.kv, kb0 = it.kb0;
             const int b = kv / p.hkv_local, kvl = kv % p.hkv_local;
-            const int used = (it.sk + P - 1) / P;  // pages that hold this sequence's keys
+            int used = (it.sk + P - 1) / P;  // pages that hold this sequence's keys ...
+            int first = 0;
+            if constexpr (MOD != 0) {  // ... of the item's first block to its last: what else the table holds is not read
+                first = kb0 / P;
+                used = min(used, (kb0 + (it.nblk + it.skip) * kBN - 1) / P + 1);
+            }
             const int *row = p.block_table + (size_t)b * p.max_pages;
             if (lane == 0) {
                 if (qi > 0 && !mbar_wait(q_empty, (qi - 1) & 1, abort_flag, p.status, kDevErrTimeoutQ, p.gen)) ok = false;
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 const int pg_lo = key0 / P, pg_hi = (key0 + kBN - 1) / P;
                 if (win_base < 0 || pg_hi >= win_base + C::PID_WIN || (MOD >= kModBias && pg_lo < win_base)) {  // warp-uniform
                     win_base = pg_lo;
-                    if (MOD >= kModBias && (i >> 1) <= it.near) win_base = max(0, pg_hi - C::PID_WIN + 1);  // going back
+                    if (MOD >= kModBias && (i >> 1) <= it.near) win_base = max(first, pg_hi - C::PID_WIN + 1);  // going back
                     bool bad = false;
                     for (int e = lane; e < C::PID_WIN; e += 32) {
                         const int pg = win_base + e;

@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(kThreads, 2)
             const Span sp = seq_span<kTile>(p, b);
             const int len = sp.len, nt = sp.nt;
             const int kvh = u / p.row_blocks;
-            const int used = (int)(((long long)len + P - 1) / P);
             const int *table = p.block_table ? p.block_table + (size_t)b * p.max_pages : nullptr;
             const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
             // page ids of the next 32 chunks (a chunk: `rows` keys), one a lane
@@ -116,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     const long long key = (long long)(c0 + lane) * rows;
                     const int page = (int)(key / P);
                     id = -1;
-                    if (key < len && page < used) {
+                    if (key < sp.hi && key + rows > sp.lo) {  // (what else the table holds is not read)
                         id = ld_plan(table + page);
                         if (id < 0 || id >= p.num_pages) {
                             report_pending(p, kDevErrBadPage);

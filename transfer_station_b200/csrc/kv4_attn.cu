@@ -204,9 +204,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
             constexpr bool small = decltype(small_pages)::value;
             while (left > 0 && ok) {
                 const Span sp = seq_span<kTile>(p, b);
-                const int len = sp.len, nt = sp.nt;
+                const int nt = sp.nt;
                 const int kvh = u / p.row_blocks;
-                const int used = (len + P - 1) / P;
                 const int *table = p.block_table + (size_t)b * p.max_pages;
                 const int end = (int)((long long)nt < tile + left ? (long long)nt : tile + left);
                 // chunk ids (a chunk: `rows` keys) of the next 32 chunks, one a lane
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                         const long long key = (long long)(c0 + lane) * rows;
                         const int page = (int)(key / P);
                         id = -1;
-                        if (key < len && page < used) {
+                        if (key < sp.hi && key + rows > sp.lo) {  // (what else the table holds is not read)
                             id = ld_plan(table + page);
                             if (id < 0 || id >= p.num_pages) {
                                 report_pending(p, kDevErrBadPage);
