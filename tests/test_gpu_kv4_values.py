@@ -7,7 +7,7 @@ import torch
 
 import transfer_station_b200 as ts
 from tests.mod_util import attend
-from tests.test_gpu_kv4 import check, decode, run, table_for
+from tests.test_gpu_kv4 import cache, check, decode, run, table_for
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,27 @@ def test_small_values_behind_one_heavy_key(cuda_dev, scale, D, Hkv, Hq, equal):
     ref, tol = attend(q, k, v, torch.ones(1, 1, L, dtype=torch.bool, device=dev), [L], p_half=2.0 ** -11)
     tol += 2.0 ** -37 * v.abs().sum(2, keepdim=True).repeat_interleave(Hq // Hkv, 1)
     check(o, ref, tol)
+
+
+@pytest.mark.parametrize("e", [90, 104, 110, 118, 125])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_queries_near_the_largest_number(cuda_dev, e, D, cap):
+    """Query rows up to 2^127: their largest score takes all the weight, or under a cap every positive one has the same.
+
+    The bound: weights are 2^12 times one or nothing (under a cap e^60 apart), so what remains is 1 / l, and the sum of
+    up to 333 values in 32 bits: 2^-14 of it."""
+    dev, L, Hq, Hkv, P = cuda_dev, 333, 8, 2, 32
+    pl, table, total, k, v = cache(1, Hkv, D, [L], P, dev, e)
+    g = torch.Generator(device=dev)
+    g.manual_seed(e + D)
+    q = (torch.randn(1, Hq, 1, D, generator=g, device=dev).clamp(-3.5, 3.5).double() * 2.0 ** e).bfloat16()
+    assert torch.isfinite(q).all()
+    o, scr = run(q, pl, table, total, [L], P, ts.attn_mod(softcap=cap), torch.float32, dev)
+    assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
+    kk, vv = (t.repeat_interleave(Hq // Hkv, 1) for t in (k, v))
+    s = q.double() @ kk.transpose(-1, -2)  # [1][Hq][1][L]
+    w = (s > 0).double() if cap else (s == s.amax(-1, keepdim=True)).double()
+    w = w / w.sum(-1, keepdim=True)
+    err = (o.double() - w @ vv).abs()
+    assert (err <= 2.0 ** -14 * (w @ vv.abs())).all()

@@ -361,9 +361,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                 start[n][w][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
                 start[n][w][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
             }
+            // Held below 2^100, so that rows past 2^83 stay finite: an accumulator is a multiple of 2^-57 below 2, and scores
+            // that differ at all then lie 2^43 apart.
             const float unit = (has_cap ? p.cap_in : p.scale_log2) / kKeyUnit;
-            fac[n][0] = __shfl_sync(0xffffffffu, up, 8 * t) * unit;
-            fac[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * unit;
+            fac[n][0] = fminf(__shfl_sync(0xffffffffu, up, 8 * t) * unit, 0x1p100f);
+            fac[n][1] = fminf(__shfl_sync(0xffffffffu, up, 8 * t + 4) * unit, 0x1p100f);
         }
         // ---- this lane's query columns: keys seen, position, bias
         int lo[NT][2], hi[NT][2], pos[NT][2];
