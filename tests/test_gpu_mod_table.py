@@ -23,6 +23,14 @@ def window(table, lens, P, lo, hi, total):
     return t
 
 
+def blind(begin, end, lens):
+    """Queries that see nothing, their empty ranges at either end and outside."""
+    for b, n in enumerate(lens):
+        if begin.shape[1] > 2:
+            begin[b, 0], end[b, 0] = ((0, 0), (-9, -3), (n, n))[b]
+            begin[b, 1], end[b, 1] = ((n + 4, n + 8), (5, 5), (2 ** 31 - 1, -2 ** 31))[b]
+
+
 @pytest.mark.parametrize("P", [8, 16, 64, 128, 256])
 @pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 3), (24, 2, 3), (4, 2, 40), (8, 2, 200)])
 @pytest.mark.parametrize("cap,bias", [(0.0, 0), (30.0, 0), (0.0, 1), (20.0, 1)])
@@ -38,9 +46,11 @@ def test_bf16_pages_outside_the_ranges(cuda_dev, P, Hq, Hkv, Sq, cap, bias):
     for begin, end in ((n.view(B, 1) - Sq + i - 300, n.view(B, 1) - Sq + i + 1),
                        (n.view(B, 1) // 2 - 200 + i, n.view(B, 1) // 2 + 77 + 0 * i)):
         begin, end = begin.contiguous(), end.contiguous()
+        blind(begin, end, lens)
         seen = visible(B, Sq, lens, 0, begin, end, Sk, dev)
-        lo = [int(b.clamp(min=0).min()) // 128 * 128 for b in begin]
-        hi = [(int(e.max()) + 127) // 128 * 128 for e in end]
+        some = [seen[b].any(0).nonzero() for b in range(B)]
+        lo = [int(x.min()) // 128 * 128 for x in some]
+        hi = [(int(x.max()) + 128) // 128 * 128 for x in some]
         t = window(table, lens, P, lo, hi, total)
         mod = ts.attn_mod(softcap=cap, slopes=sl, key_begin=begin, key_end=end)
         o, scr = torch.full((B, Hq, Sq, D), float("nan"), device=dev), scratch(D, dev)
@@ -66,9 +76,11 @@ def test_4_bit_pages_outside_the_ranges(cuda_dev, P, D, Hq, Hkv, Sq):
     for begin, end in ((n.view(B, 1) - Sq + i - 300, n.view(B, 1) - Sq + i + 1),
                        (n.view(B, 1) // 2 - 200 + i, n.view(B, 1) // 2 + 77 + 0 * i)):
         begin, end = begin.contiguous(), end.contiguous()
-        t = window(table, lens, P, [int(b.clamp(min=0).min()) for b in begin], [int(e.max()) for e in end], total)
+        blind(begin, end, lens)
+        seen = visible(B, Sq, lens, 0, begin, end, k.shape[2], dev)
+        some = [seen[b].any(0).nonzero() for b in range(B)]
+        t = window(table, lens, P, [int(x.min()) for x in some], [int(x.max()) + 1 for x in some], total)
         o, scr = run_kv4(q, pl, t, total, lens, P, ts.attn_mod(key_begin=begin, key_end=end), torch.float32, dev)
         assert ts.attn_flash_status(scr) == (ts.ATTN_OK, 0)
-        seen = visible(B, Sq, lens, 0, begin, end, k.shape[2], dev)
         ref, tol = attend(q, k, v, seen, lens, p_half=2.0 ** -10, p_abs=2.0 ** -26)
         check(o, ref, tol)

@@ -325,15 +325,16 @@ __global__ void __launch_bounds__(TcConfig<DP, NQT>::THREADS, 1)
                 for (int i = 0; i < p.Sq; ++i) {
                     const int b0 = p.key_begin ? ld_plan(p.key_begin + at + i) : 0;
                     const int b1 = p.key_end ? ld_plan(p.key_end + at + i) : it.sk;
-                    if (b0 < b1) {
-                        lo = min(lo, b0);
-                        hi = max(hi, b1);
+                    const int x0 = max(b0, 0), x1 = min(b1, p.causal ? min(it.sk, it.sk_total - p.Sq + i + 1) : it.sk);
+                    if (x0 < x1) {
+                        lo = min(lo, x0);
+                        hi = max(hi, x1);
                     }
                     lo1 = max(lo1, b0);
                     hi1 = min(hi1, b1);
                 }
-                it.ulo = max(0, lo);
-                it.uhi = min(it.uhi, hi);
+                it.ulo = lo;
+                it.uhi = hi;
                 it.ilo = lo1;
                 it.ihi = hi1;
             }

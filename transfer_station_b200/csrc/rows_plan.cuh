@@ -78,11 +78,15 @@ __device__ __forceinline__ Span seq_span(const RowsParams &p, int b) {
         int lo = s.len, hi = 0;
         for (int i = 0; i < p.Sq; ++i) {
             const size_t at = (size_t)b * p.Sq + i;
-            lo = min(lo, p.key_begin ? ld_plan(p.key_begin + at) : 0);
-            hi = max(hi, p.key_end ? ld_plan(p.key_end + at) : s.len);
+            const int x0 = p.key_begin ? max(ld_plan(p.key_begin + at), 0) : 0;
+            int x1 = p.key_end ? min(ld_plan(p.key_end + at), s.len) : s.len;
+            if (p.causal) x1 = min(x1, s.len - p.Sq + i + 1);
+            if (x0 >= x1) continue;  // (sees none)
+            lo = min(lo, x0);
+            hi = max(hi, x1);
         }
-        s.lo = max(lo, 0);
-        s.hi = min(hi, s.len);
+        s.lo = lo;
+        s.hi = hi;
     }
     s.t0 = s.lo / TILE;
     s.nt = s.hi > s.lo ? (s.hi + TILE - 1) / TILE - s.t0 : 1;
