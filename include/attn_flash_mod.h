@@ -38,7 +38,9 @@ extern "C" {
 #define ATTN_SOFTCAP_MAX 1e6f
 
 /* How scores are modified. The struct is read during the call; its arrays are device memory that the
- * work on the stream reads. All zero: plain attention (then identical to attn_flash_stream_out). */
+ * work on the stream reads. No cap, slopes or ranges: plain attention. Over contiguous K/V that is then
+ * attn_flash_stream_out, bit for bit, whose masked keys all have zero weights: an infinity or NaN in the value of
+ * a key past the causal limit may reach the rows of its unit there. */
 typedef struct attn_mod {
     float softcap;        /* 0, or within [ATTN_SOFTCAP_MIN, ATTN_SOFTCAP_MAX] */
     int causal;           /* nonzero: key j is seen only when j <= pos_i */

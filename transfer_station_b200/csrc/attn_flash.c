@@ -384,6 +384,8 @@ int attn_flash_mod_paged_stream(const uint16_t *Q, const uint16_t *K_pages, cons
     ts_fill(&p, Q, K_pages, V_pages, B * Hq, B * Hkv, Sq, max_pages * page_size, D, 0, 0);
     const int mrc = ts_set_mod(&p, mod, Hkv);
     if (mrc != ATTN_OK) return mrc;
+    /* (the plain kernels multiply what lies behind a sequence's end by zero: a NaN there would reach its rows) */
+    if (!p.mod) p.mod = 1;
     if (rc != ATTN_OK) return rc;
     p.O = (float *)O;
     p.o_bf16 = out_dtype == ATTN_OUT_BF16;
