@@ -47,13 +47,13 @@ __device__ __forceinline__ void cap_near(float (&s)[4], const float (&k)[5], con
         s[h] = z.x, s[h + 1] = z.y;
     }
 }
+// For a warp that holds a score past the polynomial's interval. The others' bits are cap_near's: whether a warp comes
+// here may hang on a slot that no row sees, whose score is replaced later and whose content may be anything.
 __device__ __forceinline__ void cap_any(float (&s)[4], const float (&k)[5], float cap_out, const float (&ref)[2]) {
+    const float y[4] = {s[0], s[1], s[2], s[3]};
+    cap_near(s, k, ref);
 #pragma unroll
-    for (int h = 0; h < 4; h += 2) {
-        const float2 y = make_float2(s[h], s[h + 1]), z = __fmul2_rn(y, tanh_poly(__fmul2_rn(y, y), k));
-        s[h] = cap_far(y.x, z.x, cap_out) - ref[0];
-        s[h + 1] = cap_far(y.y, z.y, cap_out) - ref[1];
-    }
+    for (int e = 0; e < 4; ++e) s[e] = cap_far(y[e], s[e], cap_out, -ref[e & 1]);
 }
 __device__ __forceinline__ void scale_less(float (&s)[4], const float (&fac)[2], const float (&ref)[2]) {
 #pragma unroll
