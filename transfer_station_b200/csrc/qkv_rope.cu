@@ -11,7 +11,7 @@
 // matter how long the consumers take. Eight consumer warps take each stage (the norm weights
 // sit in shared memory as fp32, loaded once per CTA): a head vector is
 // handled by G = D/16 lanes, 16 elements (two 16-byte shared loads) each; results go straight
-// to global memory with 16-byte stores. Each warp releases the stage as soon as its bytes are
+// to global memory with 16-byte stores. Each warp releases the stage once its bytes are
 // in registers. A CTA streams one contiguous run of chunks, so a lane meets each token once in
 // a row: the per-token work (position, destination rows, validity, the lane's cos/sin slice)
 // runs only when the token changes, and the per-vector work is the arithmetic itself. The
@@ -222,10 +222,6 @@ __global__ void __maxnreg__(72) qkv_rope_kernel(ts_rope_problem a) {
         for (int j = 0; j < PER; ++j) {
             const uint4 raj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + oa * 2);
             const uint4 rbj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + ob * 2);
-            if (j == PER - 1) {  // the stage's last bytes are in registers: release it
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty0 + 8 * st);
-            }
             const bool act = vbase + (long long)j * NG < a.n_vec;
             if (act && t != T.t) load_token<D, PAGED>(a, T, t, li, rot_lane);
             const int kind = h < a.Hq ? 0 : (h < a.Hq + a.Hkv ? 1 : 2);  // q, k, v head
@@ -239,6 +235,14 @@ __global__ void __maxnreg__(72) qkv_rope_kernel(ts_rope_problem a) {
             for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
             for (int o = G / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o, G);
+            if (j == PER - 1) {
+                // The sums above needed every lane's elements: the stage's last bytes are in registers. The fence
+                // orders these reads before the copy that refills the stage: an arrival alone overtakes loads that
+                // wait behind this warp's stores, and the next chunk's bytes took their place.
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty0 + 8 * st);
+            }
             if (kind == 0 ? has_qn : (kind == 1 && has_kn)) {
                 const float r = rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
                 const float *w = kind == 0 ? wq : wk;
