@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 else
                     second(std::true_type{});
             }
+            fence_proxy_async_smem();  // this stage's reads before the copies that refill it
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(st));
             if (++st == C::NS) {

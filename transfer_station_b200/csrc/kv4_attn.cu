@@ -613,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                     }
                 }
             }
+            fence_proxy_async_smem();  // this stage's reads before the copies that refill it
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(st));
             if (++st == C::NS) {
