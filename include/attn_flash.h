@@ -128,6 +128,9 @@ int attn_flash_stream_out(const uint16_t *Q, const uint16_t *K, const uint16_t *
  * pages block_table[b * max_pages + 0 ..] and it has seq_lens[b] of them (clamped to
  * [0, max_pages * page_size]; a sequence with none gets zero rows). block_table and seq_lens
  * are device int arrays. causal: query i of sequence b sees keys 0 .. seq_lens[b] - Sq + i.
+ * Rows of a page past the sequence's end, and keys past a row's causal limit, get weight zero in the
+ * product with V: they must hold finite numbers there (a cache that is cleared once does;
+ * attn_flash_mod_paged_stream, attn_flash_mod.h, takes any content, without modifiers too).
  * page_size is 8, 16, 32, 64 or a multiple of 128; D a multiple of 8 up to 128; all pointers
  * 16-byte aligned. A page id outside [0, num_pages) is caught by the kernel: it stops and
  * attn_flash_status returns ATTN_ERR_DEVICE. Scratch as for attn_flash_stream. */
