@@ -222,9 +222,6 @@ __global__ void __maxnreg__(72) qkv_rope_kernel(ts_rope_problem a) {
         for (int j = 0; j < PER; ++j) {
             const uint4 raj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + oa * 2);
             const uint4 rbj = *reinterpret_cast<const uint4 *>(stage + (size_t)j * NG * (D * 2) + ob * 2);
-            const bool act = vbase + (long long)j * NG < a.n_vec;
-            if (act && t != T.t) load_token<D, PAGED>(a, T, t, li, rot_lane);
-            const int kind = h < a.Hq ? 0 : (h < a.Hq + a.Hkv ? 1 : 2);  // q, k, v head
             float x[16];
             unpack8(raj, x);
             unpack8(rbj, x + 8);
@@ -236,13 +233,17 @@ __global__ void __maxnreg__(72) qkv_rope_kernel(ts_rope_problem a) {
 #pragma unroll
             for (int o = G / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o, G);
             if (j == PER - 1) {
-                // The sums above needed every lane's elements: the stage's last bytes are in registers. The fence
-                // orders these reads before the copy that refills the stage: an arrival alone overtakes loads that
-                // wait behind this warp's stores, and the next chunk's bytes took their place.
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty0 + 8 * st);
+                // Released once every lane's elements are in registers, before the token's own loads: an arrival
+                // overtakes loads that wait behind this warp's stores, and the next chunk's bytes took their place.
+                // The shuffles needed the elements of all lanes, and the barrier's address hangs on their sum (of
+                // squares, never below zero), so the arrival cannot be issued before. (After the token's loads, with a
+                // proxy fence: 65,536 tokens of 80 heads of 128 554 us, here 538.)
+                const uint32_t bar = empty0 + 8 * (ss < 0.f ? kRopeStages : st);
+                if (lane == 0) mbar_arrive(bar);
             }
+            const bool act = vbase + (long long)j * NG < a.n_vec;
+            if (act && t != T.t) load_token<D, PAGED>(a, T, t, li, rot_lane);
+            const int kind = h < a.Hq ? 0 : (h < a.Hq + a.Hkv ? 1 : 2);  // q, k, v head
             if (kind == 0 ? has_qn : (kind == 1 && has_kn)) {
                 const float r = rsqrtf(__fmaf_rn(ss, 1.0f / (float)D, a.eps));
                 const float *w = kind == 0 ? wq : wk;
