@@ -40,10 +40,12 @@
 // rescales (TMEM round trips).
 //
 // Modified scores (MOD): z = cap tanh(s / cap) - slope |distance|, keys within a row's range. What is different:
-//   * The elementwise work bounds these forms, not the MMAs: a capped score takes 2.5 packed FMAs of a
-//     polynomial and a compare more than a plain one. Up to a cap of 52 the reference is the fixed cap_ref, so
-//     a capped block needs no maximum, no rescale and no second look. 32 / 8 heads, 4,096 tokens, D = 128, causal, bf16
-//     out: plain 152 us, ranges 147, bias 162, cap 190, cap and bias 226.
+//   * The elementwise work takes these forms longer than the MMAs: a capped score takes 2.5 packed FMAs of a
+//     polynomial and a compare more than a plain one. They do not fill a pipe, though (cap: issue 40%, tensor 36%):
+//     scores, softmax and the P hand-off of a tile follow one another, and eight softmax warps do not hide it. Up
+//     to a cap of 52 the reference is the fixed cap_ref, so a capped block needs no maximum, no rescale and no second
+//     look. 32 / 8 heads, 4,096 tokens, D = 128, causal, bf16 out, SM at 1.88 to 1.96 GHz: plain 158 us, ranges 157, bias
+//     165, cap 195, cap and bias 227; a window of 1,024 keys 123.
 //   * Units whose key ranges or lengths differ are sorted by their blocks, longest first (fa_mod.cu), and walked
 //     in alternating directions; blocks that none of a unit's rows sees are not walked, in front, behind or
 //     between the keys of two query heads. Nine documents in 6,007 tokens: 274 us in the units' own order, 187

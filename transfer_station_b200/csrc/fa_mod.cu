@@ -1,6 +1,6 @@
 // fa_mod.cu -- what stands around the attention kernel with modified scores: the key ranges of packed
 // documents, the bounds of a unit's ranges, the units' order by length, and the choice of the kernel form.
-// Small kernels bound by latency: 1.5 us (ranges of 4,096 tokens), 2 us each (bounds, order).
+// Small kernels bound by latency: 1.8 us (ranges of 6,007 tokens), 2 us each (bounds, order).
 #include <cuda_runtime.h>
 #include <stdint.h>
 

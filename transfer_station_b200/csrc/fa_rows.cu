@@ -10,10 +10,11 @@
 // One producer warp streams 64-key tiles by TMA (128-byte swizzle, the layout ldmatrix reads without bank
 // conflicts) into a 96 KB ring; four consumer warps take 16 keys of each, with a running maximum and an
 // accumulator of their own, merged in shared memory at a unit's end. Two such CTAs share an SM, so that one
-// streams while the other is between units (one CTA with twice the ring: 64 sequences of 300 keys 39 us, not
-// 31). The work split is rows_plan.cuh's.
+// streams while the other is between units (one CTA with twice the ring: 64 sequences of 300 keys, 16 rows, 39 us, not
+// 33). The work split is rows_plan.cuh's.
 //
-// Measured, 16 sequences of 8,192 keys, 4 rows, D = 128, cap: 52.8 us of 42.3 for the bytes (ragged lengths).
+// Measured, 16 sequences of 8,192 keys, 4 rows, D = 128, cap: 51.8 us of 42.3 for the bytes (ragged lengths); all of full
+// length 85 us, 6.3 TB/s; over pages of 8 keys 96, 16 90, 32 and more 88; 16 rows 94.
 #include <cuda_bf16.h>
 
 #include <atomic>
@@ -520,7 +521,8 @@ int run(const fa_problem *P, cudaStream_t st) {
 
 extern "C" int ts_few_rows(const fa_problem *P) {
     // More than 16 rows would read the cache twice, from L2: 16 sequences of 8,192 keys, capped, took here and
-    // in the kernel for prompts 117 and 164 us at 16 rows, 195 and 166 at 24 (one of 32,768: 47 and 55, 64 and 57).
+    // in the kernel for prompts 117 and 164 us at 16 rows, 195 and 166 at 24 (one of 32,768: 47 and 55, 64 and 57). Since
+    // then 94 here at 16 rows, and there 155 and 49 at 24, 163 at 64.
     // (As many units as descriptors find room behind the partials; key indexes look a few tiles past the end.)
     return P->mod && (long long)(P->Hq / P->Hkv) * P->Sq <= 16 && P->Hkv <= 65536 && P->Sk <= 0x7fffffff - 65536 &&
            ts_tc_supported(P);

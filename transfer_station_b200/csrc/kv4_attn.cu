@@ -30,9 +30,11 @@
 // TMA, scales by 16-byte copies); four consumer warps take 32 keys of each tile, each with its own
 // running maximum and accumulator, merged in shared memory at a unit's end.
 //
-// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 133 us, 4 of 131,072 130 us, each 571 MB
-// of cache, 4.3 TB/s; streaming the same tiles without arithmetic takes 96 us. 9 to 16 rows of a kv head in one
-// column pair (64 sequences of 8,192 keys, 16 rows): 236 us, D = 64 138; two passes of 8 took 246 and 169.
+// Measured (D = 128, 32 / 8 heads): 64 sequences of 8,192 keys 133 us, 4 of 131,072 (64 / 8 heads) 130 us, each 571 MB
+// of cache, 4.3 TB/s, with the SM at 1.965 GHz; the time follows that clock, and a call repeated for long is held to
+// 1.8 to 1.9 GHz by the power limit: 137 to 144. With a cap of 50 143 us, a bias 150, both 159; a window of half the
+// keys 77. Streaming the same tiles without arithmetic takes 96 us. 9 to 16 rows of a kv head in one
+// column pair (64 sequences of 8,192 keys, 16 rows): 243 us, D = 64 138; two passes of 8 took 246 and 169.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -58,7 +60,8 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kHead = 12.f, kMost = 15.f;  // see the weights
 // With small pages the copy engine is bound by the number of copies, and a page's 64 bytes of scales take as
 // long as its codes: up to this page size the producer's lanes fetch them. 64 sequences of 4,096 keys (32 / 8 heads,
-// D = 128), by the engine and by the lanes: pages of 8 149 and 122 us, 16 93 and 83, 32 76 and 75, 64 70 and 71.
+// D = 128), by the engine and by the lanes: pages of 8 149 and 122 us, 16 93 and 83, 32 76 and 75, 64 70 and 71. (With the
+// values at their scale 107 to 111, 86, 79, and 75 by the engine at 64.)
 constexpr int kSmallPage = 32;
 
 struct Kv4Params : RowsParams {

@@ -7,7 +7,8 @@
 // token. The arithmetic is attn_qkv_rope_paged_stream's, operation by operation, in packed fp32 pairs. It is
 // bound by instruction issue: a variant of that call's kernel (bulk copies into a ring, a lane group per
 // vector) ran 5,760 warp instructions a token of 32 + 2 * 8 heads of 128, this one 2,970; the norm and the
-// rotation are template parameters, as branches of every pass they cost 10%. 16,384 such tokens: 75 us, 353 MB.
+// rotation are template parameters, as branches of every pass they cost 10%. 16,384 such tokens: 75 to 79 us,
+// 353 MB.
 //
 // A lane owns both members of each pair it rotates (rotate-half: elements [8i, 8i+8) and [rot/2 + 8i, +8);
 // interleaved: 16 consecutive), as in qkv_rope.cu. A rotated key then crosses through the warp's shared
